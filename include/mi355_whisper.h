@@ -102,6 +102,79 @@ int mw_process_logits(struct whisper_context *ctx, const struct whisper_full_par
                       int n_draws, const double *u, float *logits_out, float *logprobs_out, float *probs_out,
                       whisper_token_data *tok_out);
 
+/* ---- decoder operators on device memory ----
+   A key / value cache in pages that any number of sequences share, the attention that reads it and a sampler, for callers
+   that drive a decoder of their own beside Whisper's.  Unlike the entry points above these take DEVICE pointers and a HIP
+   stream, launch on that stream of GPU `device` and return without waiting; the caller's current device is restored.  They
+   allocate nothing, keep nothing between calls (the workspace is the caller's, its contents need no initialisation; two
+   calls that may overlap need two) and may be captured into a graph; what a captured call reads from device memory (lengths,
+   block tables, sampler settings) may change between replays.  The structures themselves are host memory, read before the
+   call returns.  0: launched; -1: a null or inconsistent argument, -100: refused or failed, mw_last_error says why.
+
+   The cache.  Row `offset` of page `page` of head `h` is the head_dim consecutive elements at
+   page * page_stride + h * head_stride + offset * row_stride of k and v, its scales the floats at the same place of
+   k_scale and v_scale with the scale strides.  Any order of pages, heads and rows is allowed.  head_dim is 64 or 128,
+   page_size a power of two up to 32768, strides multiples of 16 bytes and bases 16-byte aligned.  Element types:
+     MW_ELEM_BF16  no scales
+     MW_ELEM_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| <= 448 scale
+     MW_ELEM_INT8  codes -127 .. 127; scale = max|x| / 127 (fp32), at least 2^-126
+   one fp32 scale per row and head, code = round to nearest even (x / scale).  A row of an 8-bit cache that holds an
+   infinity or a NaN is kept as scale NaN and codes 0: it reads back as NaN. */
+enum mw_elem { MW_ELEM_F32 = 0, MW_ELEM_BF16 = 1, MW_ELEM_E4M3 = 2, MW_ELEM_INT8 = 3 };
+struct mw_kv_cache {
+    void *k, *v;
+    float *k_scale, *v_scale; /* null for MW_ELEM_BF16 */
+    int32_t dtype;            /* enum mw_elem */
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+    int64_t page_stride, head_stride, row_stride;                   /* elements */
+    int64_t scale_page_stride, scale_head_stride, scale_row_stride; /* floats */
+};
+/* One row per token of n_seqs sequences, back to back: sequence b owns rows cu_rows[b] .. cu_rows[b + 1] - 1 and its last row
+   is the token at position kv_len[b] - 1.  Position p of sequence b lives in page block_table[b * table_stride + p / page_size],
+   row p % page_size.  An entry outside 0 .. n_pages - 1 (a page not there yet, or given back) and positions behind
+   table_cols pages hold nothing: they are not written, read back as zeros and are invisible to the attention, as are
+   positions below zero (a sequence with more rows than kv_len).  Rows behind the last sequence are left as they are.
+   Sequences may be empty, and may share pages; a slot that two rows of one write name holds undefined values afterwards. */
+struct mw_kv_batch {
+    int32_t n_seqs, n_rows;
+    const int32_t *cu_rows;     /* [n_seqs + 1], not decreasing */
+    const int32_t *kv_len;      /* [n_seqs] tokens of the sequence, the batch's rows included */
+    const int32_t *block_table; /* [n_seqs][table_cols] */
+    int64_t table_stride;
+    int32_t table_cols;
+    int32_t max_rows, max_kv;   /* what cu_rows and kv_len are expected to reach: used to shape the launch, never for what is computed */
+};
+/* rows of keys and values (dtype MW_ELEM_F32 or MW_ELEM_BF16; head h of row t at t * row_stride + h * head_stride elements, strides
+   and bases 16-byte aligned) -> the pages */
+int mw_kv_write_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int dtype,
+                       const void *k, const void *v, int64_t row_stride, int64_t head_stride);
+/* the pages' contents at the batch's rows -> k, v (layout as above): code * scale, rounded once to dtype */
+int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int dtype,
+                      void *k, void *v, int64_t row_stride, int64_t head_stride);
+/* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the keys j of the row's sequence that its token sees: those at its
+   position p and before it; with window > 0 only j > p - window and the first `sinks` positions.  Query head h reads key /
+   value head h / (n_heads / n_kv_heads).  q and out: bf16, head h of row t at t * stride + h * head_stride, 16-byte aligned.
+   Scores, softmax and sums in fp32; the probabilities are rounded to bf16 for the product with v.  A row that sees nothing
+   is zero.  Invisible keys and values are never used, whatever they hold.  scale > 0, finite.  workspace: at least
+   mw_kv_attend_workspace bytes for the same device, cache, batch and n_heads (may be 0 bytes), 16-byte aligned. */
+size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads);
+int mw_kv_attend_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads,
+                        const void *q, int64_t q_row_stride, int64_t q_head_stride, void *out, int64_t out_row_stride,
+                        int64_t out_head_stride, float scale, int window, int sinks, void *workspace, size_t workspace_bytes);
+/* One token per row of logits (MW_ELEM_F32 or MW_ELEM_BF16, [n_rows] rows row_stride elements apart).  x = logit / temperature[row];
+   the tokens in the order (x falling, index rising); top_k keeps that many of them; top_p, of those, the fewest that hold
+   at least top_p of their probability; min_p, of those, the ones at least min_p times as likely as the likeliest; the token
+   is the first in the order of the index whose cumulated probability reaches u[row] (0 <= u < 1) of what is kept.
+   temperature <= 0: the first largest logit.  top_k <= 0, top_p >= 1 and min_p <= 0 keep all; the likeliest token is always
+   kept.  The settings are device arrays [n_rows], each may be null (temperature 1, nothing dropped).  logprobs (may be null)
+   gets log softmax(x) at the token over ALL tokens (as whisper_token_data.plog; temperature <= 0: x = logit).
+   -infinity marks a suppressed token.  A row with a NaN, a +infinity or nothing but -infinity, or whose temperature, u, top_p or
+   min_p is not a number, gives token -1 and logprob NaN.  Results do not depend on n_rows or on the other rows.
+   n_vocab <= 1048576. */
+int mw_sample_device(int device, void *stream, const void *logits, int dtype, int n_rows, int n_vocab, int64_t row_stride,
+                     const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const double *u,
+                     int32_t *ids, float *logprobs);
+
 /* ---- measurement ---- */
 struct mw_timings {
     double mel_ms, encode_ms, decode_ms, sample_ms, total_ms; /* host wall clock, cumulative */

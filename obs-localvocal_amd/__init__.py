@@ -85,6 +85,21 @@ class Timings(C.Structure):
                 ("n_sample", C.c_int)]
 
 
+ELEM_F32, ELEM_BF16, ELEM_E4M3, ELEM_INT8 = 0, 1, 2, 3
+
+
+class _KvCache(C.Structure):  # mw_kv_cache
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("dtype", C.c_int32),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("scale_page_stride", C.c_int64), ("scale_head_stride", C.c_int64), ("scale_row_stride", C.c_int64)]
+
+
+class _KvBatch(C.Structure):  # mw_kv_batch
+    _fields_ = [("n_seqs", C.c_int32), ("n_rows", C.c_int32), ("cu_rows", C.c_void_p), ("kv_len", C.c_void_p), ("block_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_cols", C.c_int32), ("max_rows", C.c_int32), ("max_kv", C.c_int32)]
+
+
 class LvDetection(C.Structure):
     _fields_ = [("result", C.c_int), ("text", C.c_char_p), ("start_timestamp_ms", C.c_uint64),
                 ("end_timestamp_ms", C.c_uint64), ("tokens", C.POINTER(TokenData)), ("n_tokens", C.c_int),
@@ -109,6 +124,7 @@ EXPORTED_SYMBOLS = [
     "mw_get_mel", "mw_encode", "mw_get_encoder_out", "mw_get_cross_kv", "mw_decode", "mw_decode_rows", "mw_get_logits", "mw_kv_clear",
     "mw_process_logits", "mw_get_timings", "mw_reset_timings", "mw_stream", "mw_synchronize",
     "mw_set_force_decode_steps", "mw_hub_stats", "mw_set_duplicate_class", "mw_bench_decode_step", "mw_bench_mel", "mw_bench_encode", "mw_last_error",
+    "mw_kv_write_device", "mw_kv_read_device", "mw_kv_attend_workspace", "mw_kv_attend_device", "mw_sample_device",
     "lv_filter_create", "lv_filter_destroy", "lv_filter_params", "lv_filter_set_language", "lv_filter_set_thresholds",
     "lv_filter_set_context_sentences", "lv_filter_push_sentence", "lv_filter_set_gpu_device", "lv_filter_load_model",
     "lv_filter_unload_model", "lv_filter_context", "lv_run_whisper_inference", "lv_to_timestamp",
@@ -209,6 +225,13 @@ def lib():
     FPm = C.POINTER(C.c_float)
     L.mw_mx_gemm.argtypes = [C.c_int, FPm, C.c_int, C.c_int, FPm, C.c_int, FPm, FPm, C.c_int, FPm, FPm, FPm]
     L.mw_mx_layernorm.argtypes = [C.c_int, FPm, FPm, FPm, C.c_int, C.c_int, FPm, FPm]
+    KC, KB, I64 = C.POINTER(_KvCache), C.POINTER(_KvBatch), C.c_int64
+    L.mw_kv_write_device.argtypes = [C.c_int, P, KC, KB, C.c_int, P, P, I64, I64]
+    L.mw_kv_read_device.argtypes = [C.c_int, P, KC, KB, C.c_int, P, P, I64, I64]
+    L.mw_kv_attend_workspace.restype = C.c_size_t
+    L.mw_kv_attend_workspace.argtypes = [C.c_int, KC, KB, C.c_int]
+    L.mw_kv_attend_device.argtypes = [C.c_int, P, KC, KB, C.c_int, P, I64, I64, P, I64, I64, C.c_float, C.c_int, C.c_int, P, C.c_size_t]
+    L.mw_sample_device.argtypes = [C.c_int, P, P, C.c_int, C.c_int, C.c_int, I64, P, P, P, P, P, P, P]
     L.mw_mel_n_len.argtypes = [P]
     L.mw_full_device.argtypes = [P, FullParams, P, C.c_int]
     L.mw_get_mel.argtypes = [P, FP]
@@ -744,3 +767,183 @@ def mx_layernorm(x, w, b, with_bf16=True, device=0):
     if rc != 0:
         raise RuntimeError(f"mw_mx_layernorm failed ({rc}): {last_error()}")
     return out, hb
+
+
+# ---- decoder operators on device memory (torch tensors; include/mi355_whisper.h says what they compute) ----
+
+def _elem(t):
+    """mw_elem of a tensor."""
+    import torch
+    e = {torch.float32: ELEM_F32, torch.bfloat16: ELEM_BF16, torch.float8_e4m3fn: ELEM_E4M3, torch.int8: ELEM_INT8}.get(t.dtype)
+    if e is None:
+        raise TypeError(f"unsupported element type {t.dtype}")
+    return e
+
+
+def _on(device, name, t, dtype=None, dim=None):
+    if t.device != device or device.type != "cuda":
+        raise ValueError(f"{name} is on {t.device}: all tensors have to be on one GPU ({device})")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}: {dtype} is needed")
+    if dim is not None and t.dim() != dim:
+        raise ValueError(f"{name} has {t.dim()} dimensions: {dim} are needed")
+
+
+def _rows(device, name, t, heads, head_dim):
+    _on(device, name, t, None, 3)
+    if t.shape[1] != heads or t.shape[2] != head_dim or (t.stride(2) != 1 and t.numel()):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, strides {t.stride()}: [rows, {heads}, {head_dim}] with adjacent elements is needed")
+
+
+def _stream(device):
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _call(what, rc):
+    if rc != 0:
+        raise RuntimeError(f"{what} failed ({rc}): {last_error()}")
+
+
+class KvBatch:
+    """The rows of a call (mw_kv_batch): sequence b owns rows cu_rows[b] .. cu_rows[b + 1] - 1, the last of them is its token at
+    position kv_len[b] - 1, and block_table[b] names its pages.  int32 tensors on the GPU, read when the call runs there;
+    max_rows and max_kv (what the two are expected to reach) only shape the launch."""
+
+    def __init__(self, cu_rows, kv_len, block_table, max_rows: int = 0, max_kv: int = 0):
+        import torch
+        d = cu_rows.device
+        _on(d, "cu_rows", cu_rows, torch.int32, 1)
+        _on(d, "kv_len", kv_len, torch.int32, 1)
+        _on(d, "block_table", block_table, torch.int32, 2)
+        n = kv_len.shape[0]
+        if cu_rows.shape[0] != n + 1 or block_table.shape[0] != n:
+            raise ValueError(f"cu_rows has {cu_rows.shape[0]} entries, kv_len {n}, block_table {block_table.shape[0]} rows: n + 1, n and n are needed")
+        if not (cu_rows.is_contiguous() and kv_len.is_contiguous()) or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            raise ValueError("cu_rows, kv_len and the rows of block_table have to be contiguous")
+        self.device, self.tensors = d, (cu_rows, kv_len, block_table)
+        self.c = _KvBatch(n, 0, cu_rows.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]),
+                          block_table.shape[1], max_rows, max_kv)
+
+    def _for(self, device, n_rows):
+        if self.device != device:
+            raise ValueError(f"the batch is on {self.device}, the cache on {device}")
+        c = _KvBatch.from_buffer_copy(self.c)  # the call's own: other threads may use the batch with other rows
+        c.n_rows = n_rows
+        return c
+
+
+class KvCache:
+    """Keys and values in pages (mw_kv_cache): k and v [pages, kv_heads, page_size, head_dim] in bfloat16, float8_e4m3fn or int8,
+    the 8-bit ones with float32 scales [pages, kv_heads, page_size].  Views with other strides (another order of pages, heads
+    and rows) are fine as long as a row's elements are adjacent."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        import torch
+        d = k.device
+        _on(d, "k", k, None, 4)
+        _on(d, "v", v, k.dtype, 4)
+        if v.shape != k.shape or v.stride() != k.stride():
+            raise ValueError("k and v have to have one shape and layout")
+        if k.stride(3) != 1:
+            raise ValueError("the elements of a row have to be adjacent")
+        e = _elem(k)
+        if e == ELEM_F32:
+            raise TypeError("a cache is bfloat16, float8_e4m3fn or int8")
+        s = (0, 0, 0)
+        if e != ELEM_BF16:
+            if k_scale is None or v_scale is None:
+                raise ValueError("an 8-bit cache needs k_scale and v_scale")
+            _on(d, "k_scale", k_scale, torch.float32, 3)
+            _on(d, "v_scale", v_scale, torch.float32, 3)
+            if k_scale.shape != k.shape[:3] or v_scale.shape != k.shape[:3] or v_scale.stride() != k_scale.stride():
+                raise ValueError("k_scale and v_scale have to be [pages, kv_heads, page_size] in one layout")
+            s = k_scale.stride()
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("a bfloat16 cache has no scales")
+        self.L, self.device, self.n_kv_heads, self.head_dim = lib(), d, k.shape[1], k.shape[3]
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.c = _KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                          v_scale.data_ptr() if v_scale is not None else None, e, k.shape[0], k.shape[2], k.shape[1], k.shape[3],
+                          k.stride(0), k.stride(1), k.stride(2), *s)
+
+    @classmethod
+    def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype, device="cuda"):
+        """An empty cache (zeros) of `dtype`."""
+        import torch
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=device).view(dtype) for _ in range(2))
+        if dtype.itemsize > 1:
+            return cls(k, v)
+        return cls(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+    def write(self, k, v, batch: KvBatch):
+        """Rows k, v [rows, kv_heads, head_dim] (float32 or bfloat16) into the pages the batch names for them."""
+        _rows(self.device, "k", k, self.n_kv_heads, self.head_dim)
+        _rows(self.device, "v", v, self.n_kv_heads, self.head_dim)
+        if v.dtype != k.dtype or v.shape != k.shape or v.stride() != k.stride():
+            raise ValueError("k and v have to have one type, shape and layout")
+        _call("mw_kv_write_device", self.L.mw_kv_write_device(self.device.index, _stream(self.device), C.byref(self.c), C.byref(batch._for(self.device, k.shape[0])),
+                                                              _elem(k), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)))
+
+    def read(self, batch: KvBatch, n_rows: int, dtype, out=None):
+        """The batch's n_rows rows as (k, v) [rows, kv_heads, head_dim] of `dtype`; out: two tensors to fill instead of new ones
+        (rows behind the last sequence are left as they are: in new ones their contents are undefined)."""
+        import torch
+        if out is None:
+            k, v = (torch.empty((n_rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
+        else:
+            k, v = out
+            _rows(self.device, "out[0]", k, self.n_kv_heads, self.head_dim)
+            _rows(self.device, "out[1]", v, self.n_kv_heads, self.head_dim)
+            if k.shape[0] != n_rows or k.dtype != dtype or v.dtype != dtype or v.shape != k.shape or v.stride() != k.stride():
+                raise ValueError("out has to be two tensors of n_rows rows in one type and layout")
+        _call("mw_kv_read_device", self.L.mw_kv_read_device(self.device.index, _stream(self.device), C.byref(self.c), C.byref(batch._for(self.device, n_rows)),
+                                                            _elem(k), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)))
+        return k, v
+
+    def attend(self, q, batch: KvBatch, scale=None, window: int = 0, sinks: int = 0, out=None):
+        """Attention of rows q [rows, heads, head_dim] (bfloat16) over their sequences' keys and values; scale defaults to
+        head_dim ** -0.5.  Rows behind the last sequence are left as they are (undefined without `out`).  The workspace
+        is a tensor of the current stream's, or of the graph that captures the call."""
+        import torch
+        _on(self.device, "q", q, torch.bfloat16, 3)
+        heads = q.shape[1]
+        _rows(self.device, "q", q, heads, self.head_dim)
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+        else:
+            _on(self.device, "out", out, torch.bfloat16, 3)
+            _rows(self.device, "out", out, heads, self.head_dim)
+            if out.shape[0] != q.shape[0]:
+                raise ValueError("out has another number of rows than q")
+        b = C.byref(batch._for(self.device, q.shape[0]))
+        need = self.L.mw_kv_attend_workspace(self.device.index, C.byref(self.c), b, heads)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        _call("mw_kv_attend_device", self.L.mw_kv_attend_device(
+            self.device.index, _stream(self.device), C.byref(self.c), b, heads, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
+            out.stride(1), self.head_dim ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr() if need else None, need))
+        return out
+
+
+def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """One token per row of logits [rows, vocab] (float32 or bfloat16), drawn with u [rows] (float64, 0 <= u < 1): (ids int32,
+    log probabilities float32).  temperature, top_p, min_p (float32) and top_k (int32) are per-row tensors or None."""
+    import torch
+    d, n = logits.device, logits.shape[0]
+    _on(d, "logits", logits, None, 2)
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise ValueError("the logits of a row have to be adjacent")
+    _on(d, "u", u, torch.float64, 1)
+    settings = (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32))
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=d), torch.empty(n, dtype=torch.float32, device=d)
+    for name, t, kind in (("u", u, torch.float64), *settings, ("out[0]", out[0], torch.int32), ("out[1]", out[1], torch.float32)):
+        if t is not None:
+            _on(d, name, t, kind, 1)
+            if t.shape[0] != n or not t.is_contiguous():
+                raise ValueError(f"{name} has to be contiguous with one entry per row")
+    at = [t.data_ptr() if t is not None else None for _, t, _ in settings]
+    _call("mw_sample_device", lib().mw_sample_device(d.index, _stream(d), logits.data_ptr(), _elem(logits), n, logits.shape[1], logits.stride(0), *at,
+                                                     u.data_ptr(), out[0].data_ptr(), out[1].data_ptr()))
+    return out

@@ -1,10 +1,12 @@
 // api.hip — the C ABI of libmi355_whisper.so (include/whisper.h + include/mi355_whisper.h).
 // Nothing crosses this boundary but plain pointers, sizes and PODs; no exception escapes.
+#include "decoder_ops.hpp"
 #include "engine.hpp"
 
 #include "../../include/mi355_whisper.h"
 
 #include <fstream>
+#include <map>
 #include <sys/stat.h>
 #include <mutex>
 
@@ -829,6 +831,95 @@ int mw_mx_layernorm(int device, const float *x, const float *w, const float *b, 
             MW_HIP(hipMemcpy(h.data(), dh.p, n * 2, hipMemcpyDeviceToHost));
             for (size_t i = 0; i < n; ++i) out_bf16[i] = bf16_to_f32_host(h[i]);
         }
+        return 0;
+    });
+}
+
+// ---- decoder operators on device memory (kv_cache.hip, kv_attend.hip, sampler.hip) ----
+namespace {
+// the caller's current device comes back when the call ends
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        MW_HIP(hipGetDevice(&before));
+        if (before == device) before = -1;
+        else MW_HIP(hipSetDevice(device));
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice &) = delete;
+};
+// compute units of a device, asked once (a plain table: the answer never changes)
+int compute_units(int device) {
+    static std::mutex mu;
+    static std::map<int, int> known;
+    std::lock_guard<std::mutex> l(mu);
+    auto it = known.find(device);
+    if (it != known.end()) return it->second;
+    int n = 0;
+    MW_HIP(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device));
+    return known[device] = n;
+}
+}  // namespace
+int mw_kv_write_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int dtype, const void *k,
+                       const void *v, int64_t row_stride, int64_t head_stride) {
+    if (!cache || !batch) return -1;
+    return guarded("mw_kv_write_device", [&]() {
+        check_kv_rows(*cache, *batch, dtype, k, v, row_stride, head_stride);
+        OnDevice g(device);
+        launch_kv_write(*cache, *batch, dtype, k, v, row_stride, head_stride, (hipStream_t)stream);
+        return 0;
+    });
+}
+int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int dtype, void *k, void *v,
+                      int64_t row_stride, int64_t head_stride) {
+    if (!cache || !batch) return -1;
+    return guarded("mw_kv_read_device", [&]() {
+        check_kv_rows(*cache, *batch, dtype, k, v, row_stride, head_stride);
+        OnDevice g(device);
+        launch_kv_read(*cache, *batch, dtype, k, v, row_stride, head_stride, (hipStream_t)stream);
+        return 0;
+    });
+}
+size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads) {
+    size_t need = 0;
+    if (!cache || !batch) return 0;
+    (void)guarded("mw_kv_attend_workspace", [&]() {
+        need = kv_attend_workspace(compute_units(device), *cache, *batch, n_heads);
+        return 0;
+    });
+    return need;  // refused arguments: 0, and the call itself says why
+}
+int mw_kv_attend_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads, const void *q,
+                        int64_t q_row_stride, int64_t q_head_stride, void *out, int64_t out_row_stride, int64_t out_head_stride, float scale,
+                        int window, int sinks, void *workspace, size_t workspace_bytes) {
+    if (!cache || !batch) return -1;
+    return guarded("mw_kv_attend_device", [&]() {
+        KvAttendArgs a;
+        a.n_heads = n_heads;
+        a.q = q; a.q_row = q_row_stride; a.q_head = q_head_stride;
+        a.out = out; a.o_row = out_row_stride; a.o_head = out_head_stride;
+        a.scale = scale; a.window = window; a.sinks = sinks;
+        a.ws = workspace; a.ws_bytes = workspace_bytes;
+        check_kv_attend(*cache, *batch, a);
+        OnDevice g(device);
+        launch_kv_attend(compute_units(device), *cache, *batch, a, (hipStream_t)stream);
+        return 0;
+    });
+}
+int mw_sample_device(int device, void *stream, const void *logits, int dtype, int n_rows, int n_vocab, int64_t row_stride,
+                     const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const double *u, int32_t *ids,
+                     float *logprobs) {
+    return guarded("mw_sample_device", [&]() {
+        SampleArgs a;
+        a.logits = logits; a.dtype = dtype; a.n_rows = n_rows; a.n_vocab = n_vocab; a.row_stride = row_stride;
+        a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+        a.u = u; a.ids = ids; a.logprobs = logprobs;
+        check_sample(a);
+        if (n_rows == 0) return 0;
+        OnDevice g(device);
+        launch_sample(a, (hipStream_t)stream);
         return 0;
     });
 }

@@ -1,0 +1,453 @@
+// kv_attend.hip — attention of each sequence's new tokens over its paged keys and values.
+//
+//   out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j,   j <= p(t),  and with a window j > p(t) - window or j < sinks
+//
+// One pass over the keys with the running maximum m and sum l of the softmax; base-2 exponents (scale log2(e) is folded
+// into the scores).  Everything is computed transposed, so that no operand changes lanes:
+//   S^T[key][row] = K . Q^T    A = K (lane: key l & 15, 8 dims), B = Q (lane: row l & 15, 8 dims; registers)
+//                              -> lane (row = l & 15, g = l >> 4) holds keys 4g .. 4g + 3 of a 16-key tile
+//   O^T[dim][row] += V^T . P^T B = P^T: the 4 + 4 probabilities a lane has of two key tiles ARE its fragment if the contraction
+//                              index of 32 keys is ordered (g, tile, r); A = V^T in that order is what two transposing LDS
+//                              reads (ds_read_tr16_b64) give from V rows as they lie in the cache
+// A "row" is one (token, query head) pair; the query heads that share a key / value head are rows of one tile, so each
+// cached row is read once for all of them.
+//
+// 8-bit caches: the codes become bf16 exactly (e4m3 has 4 significant bits, int8 codes 8) and go through the same products;
+// a key's scale multiplies its scores, a value's scale its probabilities, both in fp32.
+#include "decoder_ops.hpp"
+
+namespace mw {
+
+namespace {
+
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+
+constexpr int BF16 = MW_ELEM_BF16, E4M3 = MW_ELEM_E4M3, INT8 = MW_ELEM_INT8;
+
+struct AttendP {
+    KvView V;
+    int n_heads, group;  // query heads per key / value head
+    const bf16_t *q;
+    int64_t q_row, q_head;
+    bf16_t *out;
+    int64_t o_row, o_head;
+    float c;  // scale log2(e)
+    int window, sinks, splits;
+    float *ws_o, *ws_ml;  // [splits][n_rows][n_heads][head_dim], [splits][n_rows][n_heads][2]
+};
+
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+
+// 8 cache elements -> 8 bf16
+template <int KIND> struct Raw { using type = u32x2; };
+template <> struct Raw<BF16> { using type = u32x4; };
+template <int KIND> __device__ __forceinline__ u32x4 to_bf16(typename Raw<KIND>::type r) {
+    if constexpr (KIND == BF16) {
+        return r;
+    } else if constexpr (KIND == E4M3) {
+        return u32x4{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x, 1.0f, false)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.x, 1.0f, true)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.y, 1.0f, false)),
+                     __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.y, 1.0f, true))};
+    } else {
+        u32x4 o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned w = i < 2 ? r.x : r.y;
+            const int s = (i & 1) * 16;
+            o[i] = pack_bf16((float)(signed char)(w >> s), (float)(signed char)(w >> (s + 8)));
+        }
+        return o;
+    }
+}
+// the n lowest of 32 bits (none below 0, all from 32 on)
+__device__ __forceinline__ unsigned low_bits(int64_t n) {
+    const int c = (int)min(max(n, (int64_t)0), (int64_t)32);
+    return c == 0 ? 0u : ~0u >> (32 - c);
+}
+__device__ __forceinline__ bool has_nonfinite(u32x4 x) {  // of 8 bf16
+    unsigned bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (unsigned)((x[i] & 0x7f80u) == 0x7f80u) | (unsigned)((x[i] & 0x7f800000u) == 0x7f800000u);
+    return bad != 0;
+}
+
+// The tile of `tile_rows` rows a workgroup has: its sequence and the first row inside it.  Sequences are cut into tiles one
+// after the other; every wave looks through 64 sequences at a time.
+__device__ __forceinline__ bool find_tile(const KvView &V, int group, int tile_rows, int tile, int &seq, int &first_row) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int s0 = 0; s0 < V.n_seqs; s0 += 64) {
+        const int b = s0 + lane;
+        int n = 0;
+        if (b < V.n_seqs) {
+            const int64_t rows = (int64_t)max(0, kv_cu(V, b + 1) - kv_cu(V, b)) * group;
+            n = (int)((rows + tile_rows - 1) / tile_rows);
+        }
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(incl, o);
+            if (lane >= o) incl += u;
+        }
+        const int all = __shfl(incl, 63);
+        if (tile - base < all) {
+            const unsigned long long m = __ballot(base + incl > tile);
+            const int l = __ffsll((unsigned long long)m) - 1;
+            seq = __builtin_amdgcn_readfirstlane(s0 + l);
+            first_row = __builtin_amdgcn_readfirstlane((tile - base - __shfl(incl - n, l)) * tile_rows);
+            return true;
+        }
+        base += all;
+    }
+    return false;
+}
+
+// The keys a tile of rows at positions p_lo .. p_hi needs, in steps of KS keys: first the sinks below the window, then the
+// window (without one: everything from 0).
+struct KeySteps {
+    int64_t lo, hi;  // main stretch (lo a multiple of KS), hi: one behind the last visible key
+    int n_sink, n;   // steps of the sinks, steps in all
+};
+template <int KS> __device__ __forceinline__ KeySteps key_steps(const KvView &V, int window, int sinks, int64_t p_lo, int64_t p_hi) {
+    KeySteps s;
+    s.hi = min(p_hi + 1, (int64_t)V.table_cols << V.shift);
+    const int64_t first = window > 0 ? max((int64_t)0, p_lo - window + 1) : 0;
+    s.lo = first / KS * KS;
+    const int64_t sink_end = window > 0 ? min(min((int64_t)sinks, s.lo), s.hi) : 0;
+    s.n_sink = (int)((max(sink_end, (int64_t)0) + KS - 1) / KS);
+    s.n = s.n_sink + (int)(max((int64_t)0, s.hi - s.lo + KS - 1) / KS);
+    return s;
+}
+template <int KS> __device__ __forceinline__ int64_t step_key(const KeySteps &s, int i) { return i < s.n_sink ? (int64_t)i * KS : s.lo + (int64_t)(i - s.n_sink) * KS; }
+
+// ------------------------------------------------------------------------------------------------------------------------
+// Tiles of 16 rows: four waves take every fourth step of 32 keys; no wave waits for another before the end.
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int RS = 32;      // keys per step
+constexpr int RW = 4;       // waves
+constexpr int VPAD = 16;    // V rows in LDS: 16 elements of padding put 8 consecutive rows on different banks for the transposing reads
+
+template <int KIND, int DH>
+__global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
+    constexpr int NS = DH / 32;        // 32-dim slices of the score product
+    constexpr int ND = DH / 16;        // 16-dim tiles of the output
+    constexpr int VLD = DH + VPAD;
+    constexpr int EB = KIND == BF16 ? 2 : 1;
+    using raw_t = typename Raw<KIND>::type;
+    __shared__ __attribute__((aligned(16))) bf16_t vt[RW][RS * VLD];
+    __shared__ float sc[RW][2 * RS];
+    __shared__ float part[RW][16][DH + 4];
+    __shared__ float ml[RW][16][2];
+    const KvView &V = A.V;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
+    const int split = blockIdx.x % A.splits;
+    const int hk = (blockIdx.x / A.splits) % V.n_kv_heads, tile = blockIdx.x / A.splits / V.n_kv_heads;
+    int seq, first;
+    if (!find_tile(V, A.group, 16, tile, seq, first)) return;
+    const int row0 = kv_cu(V, seq), nq = kv_cu(V, seq + 1) - row0;
+    const int64_t p_base = (int64_t)V.kv_len[seq] - nq;  // position of the sequence's first row
+    const int n_tile = min(16, nq * A.group - first);
+    // this lane's row; lanes behind the tile's end repeat its last row and store nothing
+    const int row = first + min(fr, n_tile - 1);
+    const int tok = row / A.group, head = hk * A.group + row % A.group;
+    const int64_t p = p_base + tok;
+    const int64_t p_lo = p_base + first / A.group, p_hi = p_base + (first + n_tile - 1) / A.group;
+    u32x4 qf[NS];
+    {
+        const bf16_t *qp = A.q + (row0 + tok) * A.q_row + head * A.q_head + 8 * g;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = *(const u32x4 *)(qp + 32 * s);
+    }
+    const KeySteps ks = key_steps<RS>(V, A.window, A.sinks, p_lo, p_hi);
+    const int i0 = (int)((int64_t)ks.n * split / A.splits), i1 = (int)((int64_t)ks.n * (split + 1) / A.splits);
+    f32x4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    const int64_t head_off = hk * V.head_stride;
+    for (int i = i0 + wave; i < i1; i += RW) {
+        const int64_t key0 = step_key<RS>(ks, i);
+        // lane -> key fr of tile 0 and of tile 1: its page; keys no row sees are not loaded
+        raw_t kr[2][NS], vr[2][NS];
+        bool dead[2];
+        int64_t off[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int64_t j = key0 + 16 * t + fr;
+            const int page = j < ks.hi ? kv_page(V, seq, j) : -1;
+            dead[t] = page < 0 || (A.window > 0 && j <= p_lo - A.window && j >= A.sinks);
+            off[t] = dead[t] ? head_off : page * V.page_stride + head_off + (j & V.mask) * V.row_stride;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                kr[t][s] = *(const raw_t *)(V.k + (off[t] + 32 * s + 8 * g) * EB);
+                vr[t][s] = *(const raw_t *)(V.v + (off[t] + 32 * s + 8 * g) * EB);
+            }
+            if constexpr (KIND != BF16) {
+                // lanes 0 .. 15 fetch the key's scale, 16 .. 31 the value's
+                if (g < 2) {
+                    const float *sp = g ? V.vs : V.ks;
+                    const int64_t so = dead[t] ? hk * V.s_head : page * V.s_page + hk * V.s_head + (j & V.mask) * V.s_row;
+                    sc[wave][g * RS + 16 * t + fr] = sp[so];
+                }
+            }
+        }
+        // V rows -> LDS (dead ones as zeros)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                u32x4 x = to_bf16<KIND>(vr[t][s]);
+                if (dead[t]) x = u32x4{0, 0, 0, 0};
+                *(u32x4 *)&vt[wave][(16 * t + fr) * VLD + 32 * s + 8 * g] = x;
+            }
+        __builtin_amdgcn_wave_barrier();  // what other lanes of the wave read below is written above (LDS keeps a wave's order)
+        // scores
+        float s[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < NS; ++c)
+                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, to_bf16<KIND>(kr[t][c])), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] = a[r] * (KIND == BF16 ? A.c : sc[wave][16 * t + 4 * g + r] * A.c);
+        }
+        // the 32 keys this lane's row sees, a bit each
+        unsigned vis = ~(unsigned)(__ballot(dead[0]) & 0xffff) & ~((unsigned)(__ballot(dead[1]) & 0xffff) << 16);
+        vis &= low_bits(p - key0 + 1);
+        if (A.window > 0) vis &= ~low_bits(p - A.window - key0 + 1) | low_bits((int64_t)A.sinks - key0);
+        const bool whole = __ballot(vis != ~0u) == 0;
+        const unsigned mine = vis >> (4 * g);  // bit 16 t + r: the lane's key r of tile t
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][r] = mine & (1u << (16 * t + r)) ? s[t][r] : -INFINITY;
+        }
+        // running maximum and sum
+        float mx = m;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
+        mx = xor_max<32>(xor_max<16>(mx));
+        const float ref = mx == -INFINITY ? 0.0f : mx;  // nothing seen so far: exp2(-inf - 0) = 0
+        const float corr = __builtin_amdgcn_exp2f(m - ref);
+        m = mx;
+        float ps = 0.0f;
+        float pv[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(s[t][r] - ref);
+                ps += e;
+                // (the scale of a value that is not seen may be anything)
+                if constexpr (KIND == BF16) pv[t][r] = e;
+                else pv[t][r] = mine & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
+            }
+        l = l * corr + ps;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= corr;
+        bool per_key = false;
+        if (KIND != INT8 && !whole) {  // a value that some rows see and others do not must not reach the others: 0 x inf = NaN
+            bool bad = false;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int c = 0; c < NS; ++c) bad |= !dead[t] && has_nonfinite(to_bf16<KIND>(vr[t][c]));
+            per_key = __ballot(bad) != 0;
+        }
+        if (!per_key) {
+            const u32x4 pb = {pack_bf16(pv[0][0], pv[0][1]), pack_bf16(pv[0][2], pv[0][3]), pack_bf16(pv[1][0], pv[1][1]), pack_bf16(pv[1][2], pv[1][3])};
+            const bf16_t *vb = &vt[wave][(4 * g + (fr >> 2)) * VLD + (fr & 3) * 4];
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * d)));
+                const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * VLD + 16 * d)));
+                const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+            }
+        } else {  // key by key, rows that see it only (part is free until the end)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) (&part[wave][0][0])[(16 * t + 4 * g + r) * 16 + fr] = __uint_as_float(pack_bf16(pv[t][r], 0.0f) << 16);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int k = 0; k < RS; ++k) {
+                const float pk = (&part[wave][0][0])[k * 16 + fr];
+                const bf16_t *vrow = &vt[wave][k * VLD + 4 * g];
+                const bool ok = (vis >> k) & 1;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = fmaf(pk, __uint_as_float((unsigned)vrow[16 * d + e] << 16), o[d][e]);
+                        o[d][e] = ok ? x : o[d][e];
+                    }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();  // the next step's rows come after this one's reads
+    }
+    l = xor_sum<32>(xor_sum<16>(l));
+    // join the four waves
+    if (g == 0) {
+        ml[wave][fr][0] = m;
+        ml[wave][fr][1] = l;
+    }
+    __syncthreads();
+    float M = ml[0][fr][0];
+#pragma unroll
+    for (int w = 1; w < RW; ++w) M = fmaxf(M, ml[w][fr][0]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    const float f = __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *(f32x4 *)&part[wave][fr][16 * d + 4 * g] = o[d] * f;
+    __syncthreads();
+    // 256 threads: row threadIdx / 16, DH / 16 dims each
+    constexpr int E = DH / 16;
+    const int r = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * E;
+    if (r >= n_tile) return;
+    float Mr = ml[0][r][0];
+#pragma unroll
+    for (int w = 1; w < RW; ++w) Mr = fmaxf(Mr, ml[w][r][0]);
+    const float rr = Mr == -INFINITY ? 0.0f : Mr;
+    float L = 0.0f, acc[E] = {};
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+        L += ml[w][r][1] * __builtin_amdgcn_exp2f(ml[w][r][0] - rr);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += part[w][r][d0 + e];
+    }
+    const int rw = first + r, tk = rw / A.group, hd = hk * A.group + rw % A.group;
+    if (A.splits == 1) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        bf16_t *op = A.out + (row0 + tk) * A.o_row + hd * A.o_head + d0;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *(unsigned *)(op + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+    } else {
+        const int64_t at = ((int64_t)split * V.n_rows + row0 + tk) * A.n_heads + hd;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(f32x4 *)(A.ws_o + at * DH + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+        if ((threadIdx.x & 15) == 0) *(f32x2 *)(A.ws_ml + at * 2) = f32x2{Mr, L};
+    }
+}
+
+// Joins the splits of a row: one wave per (row, head).  Splits without keys have l = 0 and m = -inf.
+constexpr int MAX_SPLITS = 64;
+template <int DH>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendP A) {
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= (int64_t)A.V.n_rows * A.n_heads) return;
+    const int t = (int)(item / A.n_heads), h = (int)(item % A.n_heads);
+    if (kv_seq_of_row(A.V, t) < 0) return;  // a row behind the last sequence
+    const int64_t step = (int64_t)A.V.n_rows * A.n_heads;
+    float m = -INFINITY, l = 0.0f;
+    if (lane < A.splits) {
+        const f32x2 x = *(const f32x2 *)(A.ws_ml + (item + lane * step) * 2);
+        m = x.x;
+        l = x.y;
+    }
+    const float M = wave_max_desc(m);
+    const float f = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.0f : M));
+    const float L = wave_sum_desc(l * f);
+    constexpr int E = DH / 64;
+    float acc[E] = {};
+    for (int s = 0; s < A.splits; ++s) {
+        const float fs = __shfl(f, s);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += fs * A.ws_o[(item + s * step) * DH + lane * E + e];
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    bf16_t *op = A.out + t * A.o_row + h * A.o_head + lane * E;
+    if constexpr (E == 2) *(unsigned *)op = pack_bf16(acc[0] * inv, acc[1] * inv);
+    else *op = (bf16_t)(pack_bf16(acc[0] * inv, 0.0f) & 0xffffu);
+}
+
+// How a call is cut up; the workspace and the launch agree because both ask here.
+struct Plan {
+    int64_t tiles;
+    int splits;
+};
+Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
+    Plan p;
+    const int group = n_heads / c.n_kv_heads;
+    p.tiles = (int64_t)b.n_rows * group / 16 + b.n_seqs;
+    // the tiles that hold rows when the sequences are as expected, their workgroups, and steps of the longest
+    const int64_t expected = (int64_t)b.n_rows * group / 16 + std::min(b.n_seqs, b.n_rows);
+    const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
+    const int64_t want = 4 * (int64_t)n_cus / wgs;
+    const int64_t most = ceil_div<int64_t>(std::max(b.max_kv, 1), 4 * RW * RS);
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)MAX_SPLITS}));
+    return p;
+}
+size_t plan_bytes(const Plan &p, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
+    return p.splits == 1 ? 0 : (size_t)p.splits * b.n_rows * n_heads * (c.head_dim + 2) * sizeof(float);
+}
+
+}  // namespace
+
+size_t kv_attend_workspace(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
+    check_kv(c, b);
+    MW_CHECK(n_heads > 0 && n_heads % c.n_kv_heads == 0, "kv attend: n_heads is a multiple of n_kv_heads");
+    if (b.n_rows == 0 || b.n_seqs == 0) return 0;
+    return plan_bytes(plan(n_cus, c, b, n_heads), c, b, n_heads);
+}
+
+void check_kv_attend(const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendArgs &a) {
+    check_kv(c, b);
+    MW_CHECK(a.n_heads > 0 && a.n_heads % c.n_kv_heads == 0, "kv attend: n_heads is a multiple of n_kv_heads");
+    MW_CHECK(a.scale > 0.0f && a.scale < INFINITY, "kv attend: scale is positive and finite");
+    MW_CHECK(a.window >= 0 && a.sinks >= 0, "kv attend: window and sinks are not negative");
+    if (b.n_rows == 0 || b.n_seqs == 0) return;
+    MW_CHECK(a.q && a.out && ((uintptr_t)a.q | (uintptr_t)a.out) % 16 == 0 && a.q_row >= 0 && a.q_head >= 0 && a.o_row >= 0 && a.o_head >= 0 &&
+                 a.q_row % 8 == 0 && a.q_head % 8 == 0 && a.o_row % 8 == 0 && a.o_head % 8 == 0,
+             "kv attend: q and out pointers and strides are multiples of 16 bytes");
+    MW_CHECK((int64_t)b.n_rows * a.n_heads < (1LL << 26), "kv attend: too many rows");  // a grid holds 2^32 threads
+}
+
+void launch_kv_attend(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendArgs &a, hipStream_t st) {
+    check_kv_attend(c, b, a);
+    if (b.n_rows == 0 || b.n_seqs == 0) return;
+    const Plan p = plan(n_cus, c, b, a.n_heads);
+    const size_t need = plan_bytes(p, c, b, a.n_heads);
+    MW_CHECK(a.ws_bytes >= need && (need == 0 || (a.ws && (uintptr_t)a.ws % 16 == 0)), "kv attend: workspace too small or not 16-byte aligned");
+    AttendP A{make_view(c, b), a.n_heads, a.n_heads / c.n_kv_heads, (const bf16_t *)a.q, a.q_row, a.q_head, (bf16_t *)a.out, a.o_row, a.o_head,
+              a.scale * 1.4426950408889634f, a.window, a.sinks, p.splits, (float *)a.ws,
+              (float *)a.ws + (size_t)p.splits * b.n_rows * a.n_heads * c.head_dim};
+    const int64_t blocks = p.tiles * c.n_kv_heads * p.splits;
+    MW_CHECK(blocks < (1LL << 24), "kv attend: too many tiles");
+    const dim3 grid((unsigned)blocks), block(64 * RW);
+#define KV_GO(KIND, DH) hipLaunchKernelGGL((attend_rows_kernel<KIND, DH>), grid, block, 0, st, A)
+#define KV_DIM(KIND)                          \
+    do {                                      \
+        if (c.head_dim == 64) KV_GO(KIND, 64); \
+        else KV_GO(KIND, 128);                \
+    } while (0)
+    if (c.dtype == BF16) KV_DIM(BF16);
+    else if (c.dtype == E4M3) KV_DIM(E4M3);
+    else KV_DIM(INT8);
+#undef KV_DIM
+#undef KV_GO
+    MW_HIP(hipGetLastError());
+    if (p.splits > 1) {
+        const dim3 jg((unsigned)ceil_div<int64_t>((int64_t)b.n_rows * a.n_heads, 4));
+        if (c.head_dim == 64) hipLaunchKernelGGL(attend_join_kernel<64>, jg, dim3(256), 0, st, A);
+        else hipLaunchKernelGGL(attend_join_kernel<128>, jg, dim3(256), 0, st, A);
+        MW_HIP(hipGetLastError());
+    }
+}
+
+}  // namespace mw
