@@ -39,7 +39,7 @@ struct AttendP {
     bf16_t *out;
     int64_t o_row, o_head;
     float c;  // scale log2(e)
-    int window, sinks, splits;
+    int window, sinks, splits, tiles;
     float *ws_o, *ws_ml;  // [splits][n_rows][n_heads][head_dim], [splits][n_rows][n_heads][2]
 };
 
@@ -68,6 +68,14 @@ template <int KIND> __device__ __forceinline__ u32x4 to_bf16(typename Raw<KIND>:
         }
         return o;
     }
+}
+// what the rounding of 8 probabilities to bf16 (hi) left, itself in bf16
+__device__ __forceinline__ u32x4 low_part(const float *e, u32x4 hi) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        o[i] = pack_bf16(e[2 * i] - __uint_as_float(hi[i] << 16), e[2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u));
+    return o;
 }
 // the n lowest of 32 bits (none below 0, all from 32 on)
 __device__ __forceinline__ unsigned low_bits(int64_t n) {
@@ -270,6 +278,7 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
         }
         if (!per_key) {
             const u32x4 pb = {pack_bf16(pv[0][0], pv[0][1]), pack_bf16(pv[0][2], pv[0][3]), pack_bf16(pv[1][0], pv[1][1]), pack_bf16(pv[1][2], pv[1][3])};
+            const u32x4 pl = low_part(&pv[0][0], pb);
             const bf16_t *vb = &vt[wave][(4 * g + (fr >> 2)) * VLD + (fr & 3) * 4];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
@@ -277,12 +286,13 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
                 const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * VLD + 16 * d)));
                 const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
             }
         } else {  // key by key, rows that see it only (part is free until the end)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) (&part[wave][0][0])[(16 * t + 4 * g + r) * 16 + fr] = __uint_as_float(pack_bf16(pv[t][r], 0.0f) << 16);
+                for (int r = 0; r < 4; ++r) (&part[wave][0][0])[(16 * t + 4 * g + r) * 16 + fr] = pv[t][r];
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
             for (int k = 0; k < RS; ++k) {
@@ -344,6 +354,272 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------------------
+// Tiles of 128 rows for chunks: four waves of 32 rows share steps of 64 keys, double-buffered in LDS.
+//
+// 32 x 32 x 16 products: lane (row = l & 31, h = l >> 5) holds of a block of 32 keys the scores of keys 8 b + 4 h + r (b, r = 0 .. 3),
+// so a row's maximum and sum are completed by one exchange with lane ^ 32, and the probabilities of 16 keys are a fragment
+// of P^T if the contraction index is ordered (h, b, r) — the order two transposing reads give V^T in.
+// The next step's rows travel global -> registers -> LDS (8-bit codes become bf16 on the way); their pages are looked up
+// one step earlier still, a key per lane.
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int CR = 128, CK = 64;  // rows, keys per step
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+
+template <int KIND, int DH>
+__global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
+    constexpr int KLD = DH + 8, VLD = DH + 16;  // row strides in LDS: fragment reads without bank conflicts
+    constexpr int EB = KIND == BF16 ? 2 : 1;
+    constexpr int LPR = DH / 8, RPP = 256 / LPR, NP = CK / RPP;  // lanes per row, rows per pass, passes
+    using raw_t = typename Raw<KIND>::type;
+    __shared__ __attribute__((aligned(16))) bf16_t kt[2][CK * KLD];
+    __shared__ __attribute__((aligned(16))) bf16_t vt[2][CK * VLD];
+    __shared__ __attribute__((aligned(16))) float sc[2][2][CK];
+    __shared__ int odd[2];  // a buffer whose values are not all finite
+    const KvView &V = A.V;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 31, h = lane >> 5;
+    // tiles with the most keys first: in a chunk the later ones
+    const int hk = blockIdx.x % V.n_kv_heads, rest = blockIdx.x / V.n_kv_heads;
+    const int split = rest % A.splits, tile = A.tiles - 1 - rest / A.splits;
+    int seq, first;
+    if (!find_tile(V, A.group, CR, tile, seq, first)) return;
+    const int row0 = kv_cu(V, seq), nq = kv_cu(V, seq + 1) - row0;
+    const int64_t p_base = (int64_t)V.kv_len[seq] - nq;
+    const int n_tile = min(CR, nq * A.group - first);
+    const int row = first + min(wave * 32 + fr, n_tile - 1);
+    const int tok = row / A.group, head = hk * A.group + row % A.group;
+    const int64_t p = p_base + tok;
+    const int64_t p_lo = p_base + first / A.group, p_hi = p_base + (first + n_tile - 1) / A.group;
+    const bool active = wave * 32 < n_tile;
+    u32x4 qf[DH / 16];
+    {
+        const bf16_t *qp = A.q + (row0 + tok) * A.q_row + head * A.q_head + 8 * h;
+#pragma unroll
+        for (int s = 0; s < DH / 16; ++s) qf[s] = *(const u32x4 *)(qp + 16 * s);
+    }
+    const KeySteps ks = key_steps<CK>(V, A.window, A.sinks, p_lo, p_hi);
+    const int i0 = (int)((int64_t)ks.n * split / A.splits), i1 = (int)((int64_t)ks.n * (split + 1) / A.splits);
+    f32x16 o[DH / 32];
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int srow = tid / LPR, sub = tid % LPR;
+    // page of key `lane` of step i, -1 when no row of the tile can see it
+    auto page_of = [&](int i) -> int {
+        if (i >= i1) return -1;
+        const int64_t j = step_key<CK>(ks, i) + lane;
+        if (j >= ks.hi || (A.window > 0 && j <= p_lo - A.window && j >= A.sinks)) return -1;
+        return kv_page(V, seq, j);
+    };
+    // whether every row of the tile sees every key of the step at key0 (pages apart)
+    auto all_see = [&](int64_t key0) { return key0 + CK - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + CK <= A.sinks); };
+    raw_t rk[NP], rv[NP];
+    float rs = 0.0f;
+    unsigned rdead = 0;  // passes whose row is not there
+    auto load = [&](int64_t key0, int page) {
+        rdead = 0;
+#pragma unroll
+        for (int s = 0; s < NP; ++s) {
+            const int r = s * RPP + srow, pg = __shfl(page, r);
+            rdead |= (pg < 0) << s;
+            const int64_t off = (pg < 0 ? 0 : pg * V.page_stride + ((key0 + r) & V.mask) * V.row_stride) + hk * V.head_stride + sub * 8;
+            rk[s] = *(const raw_t *)(V.k + off * EB);
+            rv[s] = *(const raw_t *)(V.v + off * EB);
+        }
+        if constexpr (KIND != BF16) {  // waves 0 and 1: the keys' and the values' scales, a key per lane
+            if (wave < 2) {
+                const int64_t so = (page < 0 ? 0 : page * V.s_page + ((key0 + lane) & V.mask) * V.s_row) + hk * V.s_head;
+                rs = (wave ? V.vs : V.ks)[so];
+            }
+        }
+    };
+    auto store = [&](int buf, bool check) {
+        bool bad = false;
+#pragma unroll
+        for (int s = 0; s < NP; ++s) {
+            const int r = s * RPP + srow;
+            *(u32x4 *)&kt[buf][r * KLD + sub * 8] = to_bf16<KIND>(rk[s]);
+            u32x4 x = to_bf16<KIND>(rv[s]);
+            if ((rdead >> s) & 1) x = u32x4{0, 0, 0, 0};
+            if (KIND != INT8 && check) bad |= has_nonfinite(x);
+            *(u32x4 *)&vt[buf][r * VLD + sub * 8] = x;
+        }
+        if constexpr (KIND != BF16) {
+            if (wave < 2) sc[buf][wave][lane] = rs;
+        }
+        if (KIND != INT8 && bad) odd[buf] = 1;
+    };
+    if (tid < 2) odd[tid] = 0;
+    __syncthreads();
+    int page_n = page_of(i0);
+    unsigned long long dead = __ballot(page_n < 0), dead_n = 0;
+    if (i0 < i1) {
+        const int64_t key0 = step_key<CK>(ks, i0);
+        load(key0, page_n);
+        page_n = page_of(i0 + 1);
+        store(0, !all_see(key0));
+    }
+    __syncthreads();
+    for (int i = i0; i < i1; ++i) {
+        const int cur = (i - i0) & 1;
+        const int64_t key0 = step_key<CK>(ks, i);
+        const bool more = i + 1 < i1;
+        if (more) {
+            dead_n = __ballot(page_n < 0);
+            load(step_key<CK>(ks, i + 1), page_n);
+            page_n = page_of(i + 2);
+        }
+        const bool clear = dead == 0 && all_see(key0);
+        if (active) {
+            const bf16_t *kb = kt[cur], *vb = vt[cur];
+            float s[2][16];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x16 a;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) a[r] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < DH / 16; ++c) {
+                    const u32x4 kf = *(const u32x4 *)(kb + (32 * t + fr) * KLD + 16 * c + 8 * h);
+                    a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][r] = a[r];
+            }
+            if constexpr (KIND != BF16) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const f32x4 f = *(const f32x4 *)&sc[cur][0][32 * t + 8 * b + 4 * h];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
+                    }
+            }
+            unsigned vis[2] = {~0u, ~0u};
+            if (!clear) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    unsigned v = ~(unsigned)(dead >> (32 * t)) & low_bits(p - key0 + 1 - 32 * t);
+                    if (A.window > 0) v &= ~low_bits(p - A.window - key0 + 1 - 32 * t) | low_bits((int64_t)A.sinks - key0 - 32 * t);
+                    vis[t] = v;
+                    const unsigned mine = v >> (4 * h);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[t][r] = mine & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : -INFINITY;
+                }
+            }
+            // running maximum (of the unscaled scores; the scale rides in the exponent's fma)
+            float mx = s[0][0];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+            mx = xor_max<32>(mx);
+            if (__ballot(mx > m)) {
+                const float nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.0f : nm;
+                const float corr = __builtin_amdgcn_exp2f((m - ref) * A.c);
+                m = nm;
+                l *= corr;
+#pragma unroll
+                for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] *= corr;
+            }
+            const float ref = m == -INFINITY ? 0.0f : -m * A.c;
+            float ps = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], A.c, ref));
+                    ps += s[t][r];
+                }
+            l += ps;
+            if constexpr (KIND != BF16) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const f32x4 f = *(const f32x4 *)&sc[cur][1][32 * t + 8 * b + 4 * h];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
+                    }
+                if (!clear) {  // (the scale of a value that is not seen may be anything)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[t][r] = (vis[t] >> (4 * h)) & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : 0.0f;
+                }
+            }
+            if (KIND == INT8 || clear || odd[cur] == 0) {
+                const int gi = lane >> 4, ii = lane & 15;
+                const bf16_t *va = vb + (4 * h + (ii >> 2)) * VLD + 16 * (gi & 1) + (ii & 3) * 4;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float *e = &s[c >> 1][8 * (c & 1)];
+                    const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
+                    u32x4 pl = {0, 0, 0, 0};
+                    if constexpr (KIND == INT8) pl = low_part(e, pb);
+#pragma unroll
+                    for (int d = 0; d < DH / 32; ++d) {
+                        const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + 16 * c * VLD + 32 * d)));
+                        const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + (16 * c + 8) * VLD + 32 * d)));
+                        const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+                        if constexpr (KIND == INT8)
+                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
+                    }
+                }
+            } else {
+                // values that are not finite and that some rows do not see (0 x inf = NaN): key by key, rows that see it only
+#pragma unroll 1
+                for (int k = 0; k < CK; ++k) {
+                    const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the 32 of its half
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
+                    const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
+                    const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
+                    const bf16_t *vrow = vb + k * VLD + 4 * h;
+#pragma unroll
+                    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            const float x = fmaf(pk, __uint_as_float((unsigned)vrow[32 * d + 8 * (q >> 2) + (q & 3)] << 16), o[d][q]);
+                            o[d][q] = ok ? x : o[d][q];
+                        }
+                }
+            }
+        }
+        if (more) {
+            // (the other buffer was last read before the previous barrier)
+            if (KIND != INT8 && tid == 0) odd[cur ^ 1] = 0;
+            if (KIND != INT8 && !all_see(step_key<CK>(ks, i + 1))) __syncthreads();
+            store(cur ^ 1, !all_see(step_key<CK>(ks, i + 1)));
+        }
+        dead = dead_n;
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+    if (!active || wave * 32 + fr >= n_tile) return;
+    const bool part = A.splits > 1;
+    const float inv = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t at = ((int64_t)split * V.n_rows + row0 + tok) * A.n_heads + head;
+    bf16_t *op = A.out + (row0 + tok) * A.o_row + head * A.o_head + 4 * h;
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const f32x4 x = {o[d][4 * b] * inv, o[d][4 * b + 1] * inv, o[d][4 * b + 2] * inv, o[d][4 * b + 3] * inv};
+            if (part) *(f32x4 *)(A.ws_o + at * DH + 32 * d + 8 * b + 4 * h) = x;
+            else *(u32x2 *)(op + 32 * d + 8 * b) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+        }
+    // (the join takes maxima in scaled units)
+    if (part && h == 0) *(f32x2 *)(A.ws_ml + at * 2) = f32x2{m * A.c, l};
+}
+
 // Joins the splits of a row: one wave per (row, head).  Splits without keys have l = 0 and m = -inf.
 constexpr int MAX_SPLITS = 64;
 template <int DH>
@@ -378,18 +654,22 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendP A) {
 
 // How a call is cut up; the workspace and the launch agree because both ask here.
 struct Plan {
+    int rows;  // of a tile
     int64_t tiles;
     int splits;
 };
 Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
     Plan p;
     const int group = n_heads / c.n_kv_heads;
-    p.tiles = (int64_t)b.n_rows * group / 16 + b.n_seqs;
+    const int longest = b.max_rows > 0 ? std::min(b.max_rows, b.n_rows) : ceil_div(b.n_rows, b.n_seqs);
+    const bool chunk = (int64_t)longest * group > 48;
+    p.rows = chunk ? CR : 16;
+    p.tiles = (int64_t)b.n_rows * group / p.rows + b.n_seqs;
     // the tiles that hold rows when the sequences are as expected, their workgroups, and steps of the longest
-    const int64_t expected = (int64_t)b.n_rows * group / 16 + std::min(b.n_seqs, b.n_rows);
+    const int64_t expected = (int64_t)b.n_rows * group / p.rows + std::min(b.n_seqs, b.n_rows);
     const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
-    const int64_t want = 4 * (int64_t)n_cus / wgs;
-    const int64_t most = ceil_div<int64_t>(std::max(b.max_kv, 1), 4 * RW * RS);
+    const int64_t want = (chunk ? 2 : 4) * (int64_t)n_cus / wgs;
+    const int64_t most = ceil_div<int64_t>(std::max(b.max_kv, 1), chunk ? 8 * CK : 4 * RW * RS);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)MAX_SPLITS}));
     return p;
 }
@@ -425,12 +705,16 @@ void launch_kv_attend(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, con
     const size_t need = plan_bytes(p, c, b, a.n_heads);
     MW_CHECK(a.ws_bytes >= need && (need == 0 || (a.ws && (uintptr_t)a.ws % 16 == 0)), "kv attend: workspace too small or not 16-byte aligned");
     AttendP A{make_view(c, b), a.n_heads, a.n_heads / c.n_kv_heads, (const bf16_t *)a.q, a.q_row, a.q_head, (bf16_t *)a.out, a.o_row, a.o_head,
-              a.scale * 1.4426950408889634f, a.window, a.sinks, p.splits, (float *)a.ws,
+              a.scale * 1.4426950408889634f, a.window, a.sinks, p.splits, (int)p.tiles, (float *)a.ws,
               (float *)a.ws + (size_t)p.splits * b.n_rows * a.n_heads * c.head_dim};
     const int64_t blocks = p.tiles * c.n_kv_heads * p.splits;
     MW_CHECK(blocks < (1LL << 24), "kv attend: too many tiles");
     const dim3 grid((unsigned)blocks), block(64 * RW);
-#define KV_GO(KIND, DH) hipLaunchKernelGGL((attend_rows_kernel<KIND, DH>), grid, block, 0, st, A)
+#define KV_GO(KIND, DH)                                                                            \
+    do {                                                                                           \
+        if (p.rows == CR) hipLaunchKernelGGL((attend_chunk_kernel<KIND, DH>), grid, block, 0, st, A); \
+        else hipLaunchKernelGGL((attend_rows_kernel<KIND, DH>), grid, block, 0, st, A);              \
+    } while (0)
 #define KV_DIM(KIND)                          \
     do {                                      \
         if (c.head_dim == 64) KV_GO(KIND, 64); \

@@ -1,8 +1,8 @@
 // sampler.hip — one token per row of logits: temperature, top-k, top-p, min-p and a draw with a given uniform number.
 //
 // The order of the tokens of a row is never formed by sorting.  With x = logit / temperature and d = (max x - x) log2(e), a
-// token's weight is 2^-d; weights are held as whole numbers W = floor(2^(40 - d)) in 64 bits, so that every sum is exact and
-// independent of the order it is formed in (LDS atomics included).  A token's place in the order is the 64-bit key
+// token's weight is 2^-d.  Where weights are added in an order that may change (LDS atomics) they are whole numbers, so that
+// the sums are exact; the others are formed in one fixed order.  A token's place in the order is the 64-bit key
 // (falling logit, rising index), unique in the row.
 //   1. maximum of the row;
 //   2. total weight; when top-k or top-p cut, a histogram over d in 2048 bins (count and weight of each);
@@ -11,8 +11,8 @@
 //      threshold needs the weight top-k left;
 //   4. the weight of what is kept, its share u, and the first token in the order of the index at which the running weight
 //      reaches it: wave totals, then tiles of the one wave, then lanes of the one tile.
-// One 1024-thread workgroup per row; wave w owns a contiguous piece of the row, 16 bytes a lane and load.  Rows up to 64 k
-// tokens stay in registers between the passes; longer ones are read again (from L2 / the memory-side cache).
+// One 1024-thread workgroup per row; every pass reads the row again (207 KB of 51 866 tokens: from L2 after the first).  Kept in
+// registers between the passes (56 a thread) the same code unrolled to 40 k instructions.
 #include "decoder_ops.hpp"
 
 namespace mw {
@@ -26,54 +26,50 @@ using u64 = unsigned long long;
 constexpr int ST = 1024;          // threads
 constexpr int SW = ST / 64;       // waves
 constexpr int NB = 2048;          // bins
-constexpr int LIST = 256;         // members of a bin resolved by counting
-constexpr int REG_VALS = 64;      // values a thread keeps
-constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
+constexpr int LIST = 1024;        // tokens of a list, one a thread (a place takes 10 bits beside an index)
+constexpr int FEW = 512;          // a cut of top-k up to here is looked for among the largest tokens
+constexpr int GUESS = 384;        // threads whose largest token the list of the likeliest is to hold when no top-k says how many
+constexpr double LN2 = 0.6931471805599453;
 
 struct Shared {
     u64 mass[NB], mass2[NB];
     unsigned cnt[NB], cnt2[NB];
-    u64 list_r[LIST], list_w[LIST];
-    u64 wave64[SW];
+    u64 list_r[LIST], list_w[LIST], sorted[LIST];
+    u64 wave64[SW], wave64b[SW];
+    double wave_d[SW];
+    float wave_f[SW], most[ST], bound;
     unsigned wave32[SW];
     u64 lo, hi;                   // key range of a division
     u64 cut, cut_mass;            // last kept key, weight up to and including it
     u64 found_mass;               // weight before the bin found
-    unsigned found_bin, found_before, found_count, n_list, best_i;
+    u64 kept, total;
+    unsigned found_bin, found_before, found_count, n_list;
 };
 
 // weights and keys of a row's values
 struct Row {
-    double inv;  // log2(e) / temperature
-    double max;
-    __device__ __forceinline__ float dist(float x) const { return (float)((max - (double)x) * inv); }
-    __device__ __forceinline__ int bin(float x) const { return (int)fminf(dist(x) * 64.0f, (float)(NB - 1)); }
-    // 2^-d = 2^-whole 2^-part, |part| <= 1/2: the exponential of a small number keeps its last place
-    __device__ __forceinline__ void split(float x, int &whole, float &e) const {
-        const double d = (max - (double)x) * inv;
-        const double w = rint(fmin(d, 256.0));
-        whole = (int)w;
-        e = __builtin_amdgcn_exp2f((float)(w - fmin(d, 256.0)));
-    }
+    float max, c;  // c = log2(e) / temperature
+    double c_d;
+    // -d = (x - max) log2(e) / temperature; -inf stays -inf.  Both roundings keep the order of the tokens.
+    __device__ __forceinline__ float power(float x) const { return (x - max) * c; }
+    __device__ __forceinline__ float share(float x) const { return __builtin_amdgcn_exp2f(power(x)); }  // of the likeliest token's probability
+    __device__ __forceinline__ unsigned weight32(float x) const { return (unsigned)fmaf(share(x), 2147483648.0f, 0.5f); }  // 2^31 of it, to the nearest
+    // bin b holds -64 d in (-b - 1, -b], the last one all from there on
+    // floor(2^(40 - d)), from d in 64 bits: 2^-d = 2^-whole 2^-part, |part| <= 1/2
     __device__ __forceinline__ u64 weight(float x) const {
-        int whole;
-        float e;
-        split(x, whole, e);
-        const u64 m = (u64)(unsigned)(e * 16777216.0f) << 36;  // exact: e has 24 significant bits, 0.7 <= e <= 1.42
-        return whole < 44 ? m >> (whole + 20) : 0;
+        const double d = fmin(((double)max - (double)x) * c_d, 200.0), w = rint(d);
+        const u64 m = (u64)(unsigned)(__builtin_amdgcn_exp2f((float)(w - d)) * 16777216.0f) << 36;  // 24 significant bits
+        return w < 44.0 ? m >> ((int)w + 20) : 0;
     }
-    __device__ __forceinline__ float share(float x) const {  // of the likeliest token's probability
-        int whole;
-        float e;
-        split(x, whole, e);
-        return ldexpf(e, -whole);
-    }
+    __device__ __forceinline__ float logprob(float x, double z) const { return (float)(((double)x - (double)max) * c_d * LN2 - log(z)); }
 };
-__device__ __forceinline__ u64 rank_key(float x, int i) {
-    unsigned b = __float_as_uint(x);
-    b ^= (b >> 31) ? 0xffffffffu : 0x80000000u;  // rising with x
-    return (u64)(~b) << 32 | (unsigned)i;
+__device__ __forceinline__ unsigned ordered(float x) {  // rising with x
+    const unsigned b = __float_as_uint(x + 0.0f);  // -0 and 0 are one value
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float unordered(unsigned b) { return __uint_as_float(b ^ ((b >> 31) ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ u64 rank_key(float x, int i) { return (u64)(~ordered(x)) << 32 | (unsigned)i; }
+__device__ __forceinline__ float key_value(u64 r) { return unordered(~(unsigned)(r >> 32)); }
 
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
 #pragma unroll
@@ -81,17 +77,149 @@ __device__ __forceinline__ u64 wave_sum64(u64 v) {
     return v;
 }
 
-// v summed over the workgroup; every thread gets the sum
-__device__ __forceinline__ u64 block_sum64(Shared &S, u64 v) {
-    v = wave_sum64(v);
+// a and b summed over the workgroup; every thread gets the sums
+__device__ __forceinline__ void block_sum64(Shared &S, u64 &a, u64 &b) {
+    a = wave_sum64(a);
+    b = wave_sum64(b);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) S.wave64[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) {
+        S.wave64[threadIdx.x >> 6] = a;
+        S.wave64b[threadIdx.x >> 6] = b;
+    }
     __syncthreads();
-    u64 t = 0;
+    a = b = 0;
 #pragma unroll
-    for (int w = 0; w < SW; ++w) t += S.wave64[w];
+    for (int w = 0; w < SW; ++w) {
+        a += S.wave64[w];
+        b += S.wave64b[w];
+    }
+}
+// how many threads of the workgroup say yes
+__device__ __forceinline__ int block_count(Shared &S, bool yes) {
+    const int n = __popcll(__ballot(yes));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) S.wave32[threadIdx.x >> 6] = n;
+    __syncthreads();
+    int t = 0;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) t += (int)S.wave32[w];
     return t;
 }
+// v summed over the workgroup in one order (fp32 inside a wave, 64 bits over the waves); every thread gets the sum
+__device__ __forceinline__ double block_sum_f(Shared &S, float v) {
+    v = wave_sum_desc(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) S.wave_f[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = 0.0;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) t += (double)S.wave_f[w];
+    return t;
+}
+// A value that at least `want` of the threads' largest values reach, and not many more: bisection between the row's maximum and
+// 2^-32 of its weight, by one wave (16 values a lane, counted by ballots: no barrier inside).  -FLT_MAX when that many do not
+// exist there.
+__device__ __forceinline__ float bound_of(Shared &S, float mine, const Row &R, int want) {
+    S.most[threadIdx.x] = mine;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        float v[SW];
+#pragma unroll
+        for (int i = 0; i < SW; ++i) v[i] = S.most[i * 64 + threadIdx.x];
+        auto reach = [&](float x) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < SW; ++i) n += __popcll(__ballot(v[i] >= x));
+            return n;
+        };
+        float hi = R.max, lo = fmaxf(R.max - 32.0f / R.c, -3.4028235e38f);
+        if (reach(lo) < want) {
+            lo = -3.4028235e38f;
+        } else {
+            for (int i = 0; i < 14; ++i) {
+                const float mid = 0.5f * lo + 0.5f * hi;
+                const int n = reach(mid);
+                if (n >= want) {
+                    lo = mid;
+                    if (n <= want + 8 + want / 8) break;
+                } else {
+                    hi = mid;
+                }
+            }
+        }
+        if (threadIdx.x == 0) S.bound = lo;
+    }
+    __syncthreads();
+    return S.bound;
+}
+
+template <int N> __device__ __forceinline__ u64 lane_xor64(u64 v) {
+    const unsigned lo = (unsigned)v, hi = (unsigned)(v >> 32);
+    if constexpr (N < 16) {
+        return (u64)__float_as_uint(lane_xor<N>(__uint_as_float(hi))) << 32 | __float_as_uint(lane_xor<N>(__uint_as_float(lo)));
+    } else {  // both copies go in: a lane gets its own row's (half's) value in one result and the partner's in the other
+        unsigned a, b;
+        if constexpr (N == 16) {
+            const auto p = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), q = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+            a = p[0] ^ p[1] ^ lo;
+            b = q[0] ^ q[1] ^ hi;
+        } else {
+            const auto p = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), q = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+            a = p[0] ^ p[1] ^ lo;
+            b = q[0] ^ q[1] ^ hi;
+        }
+        return (u64)b << 32 | a;
+    }
+}
+template <int STRIDE> __device__ __forceinline__ void sort_step(u64 &key, int size) {
+    if (size <= STRIDE) return;
+    const u64 o = lane_xor64<STRIDE>(key);
+    const bool low = (threadIdx.x & STRIDE) == 0, up = (threadIdx.x & size) == 0;
+    key = (low == up) == (o < key) ? o : key;
+}
+// The keys of threads 0 .. n - 1 in rising order (bitonic; strides inside a wave without LDS); the others give ~0.  Every thread
+// of the workgroup calls; n <= 64 is one wave's work without barriers.
+__device__ __forceinline__ u64 block_sort(Shared &S, u64 key, int n) {
+    const int t = threadIdx.x;
+    int N = 64;
+    while (N < n) N *= 2;
+    for (int size = 2; size <= N; size *= 2) {
+        for (int stride = size / 2; stride >= 64; stride /= 2) {
+            S.sorted[t] = key;
+            __syncthreads();
+            const u64 o = S.sorted[t ^ stride];
+            const bool low = (t & stride) == 0, up = (t & size) == 0;
+            key = (low == up) == (o < key) ? o : key;
+            __syncthreads();
+        }
+        if (t < N) {
+            sort_step<32>(key, size);
+            sort_step<16>(key, size);
+            sort_step<8>(key, size);
+            sort_step<4>(key, size);
+            sort_step<2>(key, size);
+            sort_step<1>(key, size);
+        }
+    }
+    return key;
+}
+// w summed over threads 0 .. this one; n: threads that have any
+__device__ __forceinline__ u64 block_scan(Shared &S, u64 w, int n) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 u = __shfl_up(w, o);
+        if (lane >= o) w += u;
+    }
+    __syncthreads();
+    if (lane == 63) S.wave64[wave] = w;
+    __syncthreads();
+    if (n > 64)
+        for (int q = 0; q < wave; ++q) w += S.wave64[q];
+    return w;
+}
+// the key of list entry t with its place in the list: (value, index, place) in one number; indices are below 2^20
+__device__ __forceinline__ u64 placed_key(u64 r, int place) { return (r >> 32) << 32 | (unsigned)r << 10 | (unsigned)place; }
 
 // The first bin whose running count (BY_COUNT: >= want) or running weight (>= want as doubles) is reached; bins follow each other in
 // the order of the tokens.  Results in S.found_*.
@@ -139,24 +267,23 @@ __device__ void find_bin(Shared &S, const unsigned *cnt, const u64 *mass, unsign
     __syncthreads();
 }
 
-template <bool BF, bool REG> struct Source {
+// A row's values as a thread goes through them: wave w owns a contiguous piece of the row, in rounds of 64 x 16 bytes.
+template <bool BF> struct Source {
     static constexpr int VEC = BF ? 8 : 4;
     const void *row;
-    int n, mis, nc, cpw, K, c0;  // values, values before the row in its first 16 bytes, 16-byte pieces, pieces per wave, rounds
-    float x[REG ? REG_VALS : 1];
+    int n, mis, K, c0;  // values, values before the row in its first 16 bytes, rounds, the thread's first 16-byte piece
 
     __device__ __forceinline__ void init(const void *p, int n_) {
         row = p;
         n = n_;
         mis = (int)(((uintptr_t)p & 15) / (BF ? 2 : 4));
-        nc = (n + mis + VEC - 1) / VEC;
-        cpw = ((nc + SW - 1) / SW + 63) / 64 * 64;
-        K = cpw / 64;
-        c0 = (threadIdx.x >> 6) * cpw + (threadIdx.x & 63);
+        const int nc = (n + mis + VEC - 1) / VEC;
+        K = ((nc + SW - 1) / SW + 63) / 64;
+        c0 = (threadIdx.x >> 6) * K * 64 + (threadIdx.x & 63);
     }
-    // values of piece c; what lies outside the row is -inf and never read
-    __device__ __forceinline__ void load(int c, float (&v)[VEC]) const {
-        const int i0 = c * VEC - mis;
+    __device__ __forceinline__ int first(int k) const { return (c0 + 64 * k) * VEC - mis; }
+    // the values from index i0 on; what lies outside the row is -inf and never read
+    __device__ __forceinline__ void load(int i0, float (&v)[VEC]) const {
         if (i0 >= 0 && i0 + VEC <= n) {
             if constexpr (BF) {
                 const u32x4 a = *(const u32x4 *)((const bf16_t *)row + i0);
@@ -180,49 +307,58 @@ template <bool BF, bool REG> struct Source {
                 }
             }
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] += 0.0f;  // -0 and 0 are one value
     }
-    __device__ __forceinline__ void fill() {
-        if constexpr (REG) {
-#pragma unroll
-            for (int k = 0; k < REG_VALS / VEC; ++k) {
-                float v[VEC];
-                load(k < K ? c0 + 64 * k : nc, v);  // piece nc and those behind it: nothing
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[k * VEC + e] = v[e];
-            }
+    // f(values, index of the first, round) over this thread's pieces, until it says false
+    template <typename F> __device__ __forceinline__ void pieces(F &&f) const {
+        for (int k = 0; k < K; ++k) {
+            float v[VEC];
+            load(first(k), v);
+            if (!f(v, first(k), k)) break;
         }
     }
     // f(value, index) over this thread's values in the order of the index
     template <typename F> __device__ __forceinline__ void each(F &&f) const {
-        if constexpr (REG) {
+        pieces([&](const float (&v)[VEC], int i0, int) {
 #pragma unroll
-            for (int k = 0; k < REG_VALS / VEC; ++k) {
-                if (k < K) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) f(x[k * VEC + e], (c0 + 64 * k) * VEC - mis + e);
-                }
-            }
-        } else {
-            for (int k = 0; k < K; ++k) {
-                float v[VEC];
-                load(c0 + 64 * k, v);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) f(v[e], (c0 + 64 * k) * VEC - mis + e);
-            }
-        }
+            for (int e = 0; e < VEC; ++e) f(v[e], i0 + e);
+            return true;
+        });
     }
 };
 
 // The last kept token when the order is cut at `want` (a count or a weight): S.cut (its key) and S.cut_mass (weight up to and with it).
 template <bool BY_COUNT, typename SRC>
-__device__ void resolve(Shared &S, const SRC &src, const Row &R, double want) {
+__device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R, double want) {
     find_bin<BY_COUNT>(S, S.cnt, S.mass, 0, 0, want);
     const int bin = (int)S.found_bin;
-    unsigned before = S.found_before, count = S.found_count;
-    u64 before_mass = S.found_mass;
-    u64 lo = 0, hi = ~0ull;
+    unsigned before = S.found_before;
+    u64 before_mass = S.found_mass, lo = 0, hi = ~0ull;
+    const float top = (float)(-bin) / 64.0f, end = bin == NB - 1 ? -INFINITY : (float)(-bin - 1) / 64.0f;
+    auto in_bin = [&](float x) {
+        const float q = R.power(x);  // (64 q is exact)
+        return q > end && q <= top && x > -INFINITY;
+    };
+    // the bin's members with keys lo .. hi; returns how many there are (the list holds the first LIST that came)
+    auto gather = [&]() -> unsigned {
+        __syncthreads();
+        if (threadIdx.x == 0) S.n_list = 0;
+        __syncthreads();
+        src.each([&](float x, int i) {
+            if (in_bin(x)) {
+                const u64 r = rank_key(x, i);
+                if (r >= lo && r <= hi) {
+                    const unsigned at = atomicAdd(&S.n_list, 1u);
+                    if (at < LIST) {
+                        S.list_r[at] = r;
+                        S.list_w[at] = R.weight32(x);
+                    }
+                }
+            }
+        });
+        __syncthreads();
+        return S.n_list;
+    };
+    unsigned count = gather();
     if (count > LIST) {  // the members' range of keys
         if (threadIdx.x == 0) {
             S.lo = ~0ull;
@@ -231,7 +367,7 @@ __device__ void resolve(Shared &S, const SRC &src, const Row &R, double want) {
         __syncthreads();
         u64 a = ~0ull, b = 0;
         src.each([&](float x, int i) {
-            if (x > -INFINITY && R.bin(x) == bin) {
+            if (in_bin(x)) {
                 const u64 r = rank_key(x, i);
                 a = min(a, r);
                 b = max(b, r);
@@ -254,12 +390,12 @@ __device__ void resolve(Shared &S, const SRC &src, const Row &R, double want) {
             }
             __syncthreads();
             src.each([&](float x, int i) {
-                if (x > -INFINITY && R.bin(x) == bin) {
+                if (in_bin(x)) {
                     const u64 r = rank_key(x, i);
                     if (r >= lo && r <= hi) {
                         const int b2 = (int)((r - lo) >> s);
                         atomicAdd(&S.cnt2[b2], 1u);
-                        atomicAdd(&S.mass2[b2], R.weight(x));
+                        atomicAdd(&S.mass2[b2], (u64)R.weight32(x));
                     }
                 }
             });
@@ -272,49 +408,30 @@ __device__ void resolve(Shared &S, const SRC &src, const Row &R, double want) {
             hi = min(hi, lo + ((u64)1 << s) - 1);
             __syncthreads();
         }
+        gather();
     }
-    if (threadIdx.x == 0) S.n_list = 0;
-    __syncthreads();
-    src.each([&](float x, int i) {
-        if (x > -INFINITY && R.bin(x) == bin) {
-            const u64 r = rank_key(x, i);
-            if (r >= lo && r <= hi) {
-                const unsigned at = atomicAdd(&S.n_list, 1u);
-                if (at < LIST) {
-                    S.list_r[at] = r;
-                    S.list_w[at] = R.weight(x);
-                }
-            }
-        }
-    });
-    __syncthreads();
-    const int n = (int)min(S.n_list, (unsigned)LIST);
-    if ((int)threadIdx.x < n) {
-        const u64 me = S.list_r[threadIdx.x], w = S.list_w[threadIdx.x];
-        unsigned c = before;
-        u64 m = before_mass;
-        for (int j = 0; j < n; ++j)
-            if (S.list_r[j] < me) {
-                ++c;
-                m += S.list_w[j];
-            }
-        const bool ahead = BY_COUNT ? (double)c < want : (double)m < want;
-        const bool last = BY_COUNT ? (double)(c + 1) >= want : (double)(m + w) >= want;
+    // the list in order; the cut is where the running count or weight passes `want`
+    const int n = (int)min(S.n_list, (unsigned)LIST), tid = threadIdx.x;
+    const u64 key = block_sort(S, tid < n ? placed_key(S.list_r[tid], tid) : ~0ull, n);
+    const u64 w = tid < n ? S.list_w[key & (LIST - 1)] : 0;
+    const u64 mass = before_mass + block_scan(S, w, n);
+    if (tid < n) {
+        const bool ahead = BY_COUNT ? (double)(before + tid) < want : (double)(mass - w) < want;
+        const bool last = BY_COUNT ? (double)(before + tid + 1) >= want : (double)mass >= want;
         if (ahead && last) {
-            S.cut = me;
-            S.cut_mass = m + w;
+            S.cut = (key >> 32) << 32 | ((unsigned)key >> 10);
+            S.cut_mass = mass;
         }
     }
     __syncthreads();
 }
 
-template <bool BF, bool REG>
+template <bool BF>
 __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     __shared__ Shared S;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Source<BF, REG> src;
+    Source<BF> src;
     src.init((const char *)A.logits + (int64_t)row * A.row_stride * (BF ? 2 : 4), A.n_vocab);
-    src.fill();
     const float temp = A.temperature ? A.temperature[row] : 1.0f;
     const int k = A.top_k ? A.top_k[row] : 0;
     const float top_p = A.top_p ? A.top_p[row] : 1.0f, min_p = A.min_p ? A.min_p[row] : 0.0f;
@@ -322,156 +439,244 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     const bool greedy = temp <= 0.0f;
 
     // ---- 1: maximum ----
-    for (int b = tid; b < NB; b += ST) {
-        S.cnt[b] = 0;
-        S.mass[b] = 0;
-    }
-    if (tid == 0) {
-        S.best_i = 0xffffffffu;
-        S.cut = ~0ull;
-        S.cut_mass = 0;
-    }
+    if (tid == 0) S.n_list = 0;
     float mx = -INFINITY;
-    bool bad = false;
-    src.each([&](float x, int) {
-        bad |= !(x < INFINITY);  // NaN or +inf
-        mx = fmaxf(mx, x);
-    });
+    src.each([&](float x, int) { mx = fmaxf(mx, x); });
+    const float my_max = mx;
     mx = wave_max_desc(mx);
-    bad = __ballot(bad) != 0;
-    if (lane == 0) {
-        S.wave32[wave] = __float_as_uint(mx);
-        S.wave64[wave] = bad;
-    }
+    if (lane == 0) S.wave_f[wave] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SW; ++w) {
-        mx = fmaxf(mx, __uint_as_float(S.wave32[w]));
-        bad |= S.wave64[w] != 0;
-    }
-    bad |= temp != temp || top_p != top_p || min_p != min_p || u != u || mx == -INFINITY;
-    if (bad) {  // the same for the whole workgroup
+    for (int w = 0; w < SW; ++w) mx = fmaxf(mx, S.wave_f[w]);
+    Row R;
+    R.max = mx;
+    // an infinite temperature makes all tokens equal, one so small that its reciprocal overflows leaves the largest alone
+    R.c_d = fmin(fmax(1.4426950408889634 / (greedy ? 1.0 : (double)temp), 1e-30), 1e37);
+    R.c = (float)R.c_d;
+
+    // ---- 2: total weight; the likeliest tokens into a list ----
+    const bool use_k = !greedy && k > 0 && k < A.n_vocab, use_p = !greedy && top_p < 1.0f, use_m = !greedy && min_p > 0.0f;
+    float bound = INFINITY;
+    if (greedy) bound = mx;
+    else if (use_k && k <= FEW) bound = bound_of(S, my_max, R, k);
+    else if (use_p || use_m) bound = bound_of(S, my_max, R, GUESS);
+    bound = fmaxf(bound, -3.4028235e38f);  // (-inf is never listed)
+    float zf = 0.0f;
+    src.each([&](float x, int i) {
+        zf += R.share(x);
+        if (x >= bound) {
+            const unsigned at = atomicAdd(&S.n_list, 1u);
+            if (at < LIST) S.list_r[at] = rank_key(x, i);
+        }
+    });
+    const double z = block_sum_f(S, zf);
+    // a NaN anywhere is one in the sum; with a maximum of +inf or -inf nothing can be drawn
+    if (z != z || !(mx < INFINITY) || mx == -INFINITY || temp != temp || top_p != top_p || min_p != min_p || u != u) {
         if (tid == 0) {
             A.ids[row] = -1;
             if (A.logprobs) A.logprobs[row] = __uint_as_float(0x7fc00000u);
         }
         return;
     }
-    Row R;
-    // (a temperature so small that its reciprocal overflows leaves the largest logits alone, an infinite one makes all equal)
-    R.inv = greedy ? LOG2E : LOG2E / (double)temp;
-    R.max = (double)mx;
-
-    // ---- 2: total weight, histogram ----
-    const bool use_k = !greedy && k > 0 && k < A.n_vocab, use_p = !greedy && top_p < 1.0f;
-    u64 z = 0;
-    unsigned best = 0xffffffffu;
-    src.each([&](float x, int i) {
-        if (x > -INFINITY) {
-            const u64 w = R.weight(x);
-            z += w;
-            if (x == mx) best = min(best, (unsigned)i);
-            if (use_k || use_p) {
-                const int b = R.bin(x);
-                atomicAdd(&S.cnt[b], 1u);
-                atomicAdd(&S.mass[b], w);
-            }
-        }
-    });
-    if (greedy && best != 0xffffffffu) atomicMin(&S.best_i, best);
-    z = block_sum64(S, z);
-    const double log_z = log((double)z * 0x1p-40);
-
-    int id = -1;
-    float xi = 0.0f;
-    if (greedy) {
+    const int n = (int)min(S.n_list, (unsigned)LIST);
+    if (greedy && S.n_list <= LIST) {
+        unsigned best = tid < n ? (unsigned)S.list_r[tid] : 0xffffffffu;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) best = min(best, (unsigned)__shfl_xor((int)best, o));
+        if (lane == 0) S.wave32[wave] = best;
+        __syncthreads();
         if (tid == 0) {
-            A.ids[row] = (int)S.best_i;
-            if (A.logprobs) A.logprobs[row] = (float)-log_z;
+            for (int w = 1; w < SW; ++w) best = min(best, S.wave32[w]);
+            A.ids[row] = (int)best;
+            if (A.logprobs) A.logprobs[row] = R.logprob(mx, z);
         }
         return;
     }
+    const u64 me = tid < n ? S.list_r[tid] : ~0ull;
+    const float listed_x = key_value(me);
+    const u64 w = tid < n ? R.weight(listed_x) : 0;
+    S.list_w[tid] = w;
+    // Does the list hold everything that is kept?
+    bool listed = bound < INFINITY && S.n_list <= LIST && !greedy;
+    if (listed && bound > -3.4028235e38f) {
+        if (use_k && k <= FEW) {
+            listed = n >= k;
+        } else if (use_k) {
+            listed = false;
+        } else if (use_p) {
+            u64 zb = w, t = 0;
+            block_sum64(S, zb, t);
+            listed = (double)zb >= (1.0 + 1e-6) * (double)top_p * z * 0x1p40;
+        } else {
+            listed = R.share(bound) < 0.999999f * min_p;
+        }
+    }
+    if (listed) {
+        // in the order of the tokens: what is kept is a stretch from the first on
+        u64 key = block_sort(S, tid < n ? placed_key(me, tid) : ~0ull, n);
+        const float x = key_value(key);
+        bool keep = tid < n && (!use_k || tid < k);
+        if (use_p) {
+            const u64 wt = tid < n ? S.list_w[key & (LIST - 1)] : 0, upto = block_scan(S, wt, n);
+            double kept = z * 0x1p40;
+            if (use_k) {
+                if (tid == min(k, n) - 1) S.kept = upto;
+                __syncthreads();
+                kept = (double)S.kept;
+            }
+            keep &= tid == 0 || (double)(upto - wt) < (double)top_p * kept;
+        }
+        if (use_m) keep &= x == mx || R.share(x) >= min_p;
+        const int nk = block_count(S, keep);
+        // in the order of the index: the draw
+        key = block_sort(S, tid < nk ? (u64)(unsigned)key : ~0ull, nk);
+        const u64 wi = tid < nk ? S.list_w[key & (LIST - 1)] : 0, upto = block_scan(S, wi, nk);
+        if (tid == nk - 1) S.total = upto;
+        __syncthreads();
+        const u64 total = S.total;
+        const u64 target = min(max((u64)fmin(fmax(ceil(u * (double)total), 1.0), (double)total), (u64)1), total);
+        if (tid < nk && upto - wi < target && upto >= target) {
+            A.ids[row] = (int)((unsigned)key >> 10);
+            if (A.logprobs) A.logprobs[row] = R.logprob(key_value(S.list_r[key & (LIST - 1)]), z);
+        }
+        return;
+    }
+    __syncthreads();
 
     // ---- 3: cuts ----
     u64 cut = ~0ull;
-    double kept = (double)z;
-    if (use_k) {
-        // fewer tokens than k may be left by the suppressed ones: nothing to cut then
-        unsigned live = 0;
-        {
-            unsigned c = S.cnt[2 * tid] + S.cnt[2 * tid + 1];
-            live = (unsigned)block_sum64(S, c);
+    if (greedy) cut = (u64)(~ordered(mx)) << 32 | 0x7fffffffu;  // more equal largest logits than the list holds: the first of them is drawn
+    if (use_k || use_p) {
+        for (int b = tid; b < NB; b += ST) {
+            S.cnt[b] = 0;
+            S.mass[b] = 0;
         }
-        if ((unsigned)k < live) {
-            resolve<true>(S, src, R, (double)k);
-            cut = S.cut;
-            kept = (double)S.cut_mass;
-        }
-    }
-    if (use_p) {
-        const double want = fmax((double)top_p * kept, 0.5);
         __syncthreads();
-        resolve<false>(S, src, R, want);
-        cut = S.cut;
+        // (the last bin takes all that is far away: in registers first, or its one address would be waited for by every lane)
+        unsigned far = 0;
+        u64 far_mass = 0;
+        src.each([&](float x, int) {
+            const float q = -64.0f * R.power(x);
+            if (q < (float)(NB - 1)) {
+                if (use_k) atomicAdd(&S.cnt[(int)q], 1u);
+                if (use_p) atomicAdd(&S.mass[(int)q], (u64)R.weight32(x));
+            } else if (x > -INFINITY) {
+                ++far;
+                far_mass += R.weight32(x);
+            }
+        });
+        if (far) {
+            atomicAdd(&S.cnt[NB - 1], far);
+            atomicAdd(&S.mass[NB - 1], far_mass);
+        }
+        __syncthreads();
+        double kept = z * 0x1p31;
+        if (use_k) {
+            // fewer tokens than k may be left by the suppressed ones: nothing to cut then
+            u64 live = S.cnt[2 * tid] + S.cnt[2 * tid + 1], t = 0;
+            block_sum64(S, live, t);
+            if ((u64)k < live) {
+                resolve<true>(S, src, R, (double)k);
+                cut = S.cut;
+                kept = (double)S.cut_mass;
+            }
+        }
+        if (use_p) {
+            __syncthreads();
+            resolve<false>(S, src, R, fmax((double)top_p * kept, 0.5));
+            cut = S.cut;
+        }
     }
 
     // ---- 4: draw ----
-    u64 mine = 0;
-    auto weight_kept = [&](float x, int i) -> u64 {
-        if (!(x > -INFINITY) || rank_key(x, i) > cut) return 0;
-        if (min_p > 0.0f && x != mx && R.share(x) < min_p) return 0;
-        return R.weight(x);
+    const float cut_x = cut == ~0ull ? -INFINITY : key_value(cut);
+    const int cut_i = cut == ~0ull ? 0x7fffffff : (int)(unsigned)cut;
+    constexpr int VEC = Source<BF>::VEC;
+    const float least = use_m ? fminf(min_p, 1.0f) : 0.0f;  // (the likeliest token's share is 1)
+    auto weight_kept = [&](float x, int i) -> float {
+        const float w = R.share(x);
+        const bool keep = x > cut_x || (x == cut_x && i <= cut_i);
+        return keep && w >= least ? w : 0.0f;
     };
-    src.each([&](float x, int i) { mine += weight_kept(x, i); });
-    const u64 wsum = wave_sum64(mine);
+    auto piece_kept = [&](const float (&v)[VEC], int i0) -> float {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s += weight_kept(v[e], i0 + e);
+        return s;
+    };
+    // (nothing dropped: the sums of the waves are those of step 2)
+    const bool all_kept = !use_k && !use_p && !use_m && !greedy;
+    double mine = 0.0;
+    if (!all_kept) src.pieces([&](const float (&v)[VEC], int i0, int) {
+        mine += (double)piece_kept(v, i0);
+        return true;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
     __syncthreads();
-    if (lane == 0) S.wave64[wave] = wsum;
+    if (lane == 0) S.wave_d[wave] = all_kept ? (double)S.wave_f[wave] : mine;
     __syncthreads();
-    u64 total = 0, below = 0;
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < SW; ++w) total += S.wave_d[w];
+    // The first token with which the running weight reaches u of the total.  Wave, tile and lane are found one after the other;
+    // where the last places of two sums disagree, the last one with weight is it.
+    const double target = greedy ? 0.0 : fmin(fmax(u, 0.0) * total, total);
+    double below = 0.0, run = 0.0;
+    int owner = -1;
+    bool done = false;
 #pragma unroll
     for (int w = 0; w < SW; ++w) {
-        if (w == wave) below = total;
-        total += S.wave64[w];
+        const double s = S.wave_d[w];
+        if (!done && s > 0.0) {
+            owner = w;
+            below = run;
+            done = run + s >= target;
+        }
+        run += s;
     }
-    // the first whole weight that is at least u total (at least 1: a token of weight 0 is never drawn)
-    const double want = fmin(fmax(ceil(u * (double)total), 1.0), (double)total);
-    u64 target = (u64)want;
-    target = min(max(target, (u64)1), total);
-    if (!(below < target && below + wsum >= target)) return;  // one wave goes on
-    u64 run = below;
-    for (int kk = 0; kk < src.K; ++kk) {
-        float v[Source<BF, REG>::VEC];
-        const int c = src.c0 + 64 * kk;
-        src.load(c, v);
-        u64 s = 0;
-#pragma unroll
-        for (int e = 0; e < Source<BF, REG>::VEC; ++e) s += weight_kept(v[e], c * Source<BF, REG>::VEC - src.mis + e);
-        u64 incl = s;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const u64 t = __shfl_up(incl, o);
-            if (lane >= o) incl += t;
+    if (wave != owner) return;  // one wave goes on
+    run = below;
+    int tile = 0;
+    double tile_run = below;
+    src.pieces([&](const float (&v)[VEC], int i0, int kk) {
+        const double s = (double)wave_sum_desc(piece_kept(v, i0));
+        if (s > 0.0) {
+            tile = kk;
+            tile_run = run;
         }
-        const u64 all = __shfl(incl, 63);
-        if (run + all >= target) {
-            u64 at = run + incl - s;
-            if (at < target && at + s >= target) {  // one lane
+        run += s;
+        return !(s > 0.0 && run >= target);
+    });
+    float v[VEC];
+    const int i0 = src.first(tile);
+    src.load(i0, v);
+    const double s = (double)piece_kept(v, i0);
+    double incl = s;
 #pragma unroll
-                for (int e = 0; e < Source<BF, REG>::VEC; ++e) {
-                    const int i = c * Source<BF, REG>::VEC - src.mis + e;
-                    const u64 w = weight_kept(v[e], i);
-                    if (id < 0 && w != 0 && at + w >= target) {
-                        id = i;
-                        xi = v[e];
-                    }
-                    at += w;
-                }
-                A.ids[row] = id;
-                if (A.logprobs) A.logprobs[row] = (float)(-(R.max - (double)xi) * R.inv * LN2 - log_z);
+    for (int o = 1; o < 64; o <<= 1) {
+        const double t = __shfl_up(incl, o);
+        if (lane >= o) incl += t;
+    }
+    u64 yes = __ballot(s > 0.0 && tile_run + incl >= target);
+    if (yes == 0) yes = 1ull << (63 - __clzll(__ballot(s > 0.0)));
+    if (lane == __ffsll(yes) - 1) {
+        int id = -1;
+        float xi = 0.0f;
+        double at = tile_run + incl - s;
+        bool reached = false;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float w = weight_kept(v[e], i0 + e);
+            at += (double)w;
+            if (!reached && w > 0.0f) {
+                id = i0 + e;
+                xi = v[e];
+                reached = at >= target;
             }
-            break;
         }
-        run += all;
+        A.ids[row] = id;
+        if (A.logprobs) A.logprobs[row] = R.logprob(xi, z);
     }
 }
 
@@ -492,15 +697,9 @@ void check_sample(const SampleArgs &a) {
 void launch_sample(const SampleArgs &a, hipStream_t st) {
     check_sample(a);
     if (a.n_rows == 0) return;
-    const bool reg = a.n_vocab + 8 <= SW * 64 * REG_VALS;
     const dim3 grid(a.n_rows), block(ST);
-    if (a.dtype == MW_ELEM_BF16) {
-        if (reg) hipLaunchKernelGGL((sample_kernel<true, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((sample_kernel<true, false>), grid, block, 0, st, a);
-    } else {
-        if (reg) hipLaunchKernelGGL((sample_kernel<false, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((sample_kernel<false, false>), grid, block, 0, st, a);
-    }
+    if (a.dtype == MW_ELEM_BF16) hipLaunchKernelGGL(sample_kernel<true>, grid, block, 0, st, a);
+    else hipLaunchKernelGGL(sample_kernel<false>, grid, block, 0, st, a);
     MW_HIP(hipGetLastError());
 }
 
