@@ -770,18 +770,32 @@ def mx_layernorm(x, w, b, with_bf16=True, device=0):
 
 
 # ---- decoder operators on device memory (torch tensors; include/mi355_whisper.h says what they compute) ----
+# A call of a decode step is a few microseconds on the GPU, so the checks below are written to cost little on the way to it.
+
+_ELEM = {}  # torch dtype -> mw_elem
+_torch = None
+
+
+def _load_torch():
+    """torch, imported with the first operator call (nothing else in this module needs it)."""
+    global _torch
+    if _torch is None:
+        import torch
+        _ELEM.update({torch.float32: ELEM_F32, torch.bfloat16: ELEM_BF16, torch.float8_e4m3fn: ELEM_E4M3, torch.int8: ELEM_INT8})
+        _torch = torch
+    return _torch
+
 
 def _elem(t):
     """mw_elem of a tensor."""
-    import torch
-    e = {torch.float32: ELEM_F32, torch.bfloat16: ELEM_BF16, torch.float8_e4m3fn: ELEM_E4M3, torch.int8: ELEM_INT8}.get(t.dtype)
+    e = _ELEM.get(t.dtype)
     if e is None:
         raise TypeError(f"unsupported element type {t.dtype}")
     return e
 
 
 def _on(device, name, t, dtype=None, dim=None):
-    if t.device != device or device.type != "cuda":
+    if not t.is_cuda or t.device != device:
         raise ValueError(f"{name} is on {t.device}: all tensors have to be on one GPU ({device})")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}: {dtype} is needed")
@@ -789,15 +803,19 @@ def _on(device, name, t, dtype=None, dim=None):
         raise ValueError(f"{name} has {t.dim()} dimensions: {dim} are needed")
 
 
-def _rows(device, name, t, heads, head_dim):
-    _on(device, name, t, None, 3)
-    if t.shape[1] != heads or t.shape[2] != head_dim or (t.stride(2) != 1 and t.numel()):
+def _rows(device, name, t, heads, head_dim, dtype=None):
+    """Checks a tensor of rows [rows, heads, head_dim]; returns (rows, row stride, head stride)."""
+    _on(device, name, t, dtype, 3)
+    n, h, d = t.shape
+    sr, sh, se = t.stride()
+    if h != heads or d != head_dim or (se != 1 and n):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, strides {t.stride()}: [rows, {heads}, {head_dim}] with adjacent elements is needed")
+    return n, sr, sh
 
 
 def _stream(device):
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of a GPU (a hipStream_t)."""
+    return _torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _call(what, rc):
@@ -811,19 +829,18 @@ class KvBatch:
     max_rows and max_kv (what the two are expected to reach) only shape the launch."""
 
     def __init__(self, cu_rows, kv_len, block_table, max_rows: int = 0, max_kv: int = 0):
-        import torch
+        i32 = (_torch or _load_torch()).int32
         d = cu_rows.device
-        _on(d, "cu_rows", cu_rows, torch.int32, 1)
-        _on(d, "kv_len", kv_len, torch.int32, 1)
-        _on(d, "block_table", block_table, torch.int32, 2)
-        n = kv_len.shape[0]
-        if cu_rows.shape[0] != n + 1 or block_table.shape[0] != n:
-            raise ValueError(f"cu_rows has {cu_rows.shape[0]} entries, kv_len {n}, block_table {block_table.shape[0]} rows: n + 1, n and n are needed")
-        if not (cu_rows.is_contiguous() and kv_len.is_contiguous()) or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        _on(d, "cu_rows", cu_rows, i32, 1)
+        _on(d, "kv_len", kv_len, i32, 1)
+        _on(d, "block_table", block_table, i32, 2)
+        n, (tn, cols), (ts, te) = kv_len.shape[0], block_table.shape, block_table.stride()
+        if cu_rows.shape[0] != n + 1 or tn != n:
+            raise ValueError(f"cu_rows has {cu_rows.shape[0]} entries, kv_len {n}, block_table {tn} rows: n + 1, n and n are needed")
+        if not (cu_rows.is_contiguous() and kv_len.is_contiguous()) or (cols > 1 and te != 1):
             raise ValueError("cu_rows, kv_len and the rows of block_table have to be contiguous")
         self.device, self.tensors = d, (cu_rows, kv_len, block_table)
-        self.c = _KvBatch(n, 0, cu_rows.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]),
-                          block_table.shape[1], max_rows, max_kv)
+        self.c = _KvBatch(n, 0, cu_rows.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), ts if ts > cols or n > 1 else cols, cols, max_rows, max_kv)
 
     def _for(self, device, n_rows):
         if self.device != device:
@@ -839,7 +856,7 @@ class KvCache:
     and rows) are fine as long as a row's elements are adjacent."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
-        import torch
+        torch = _load_torch()
         d = k.device
         _on(d, "k", k, None, 4)
         _on(d, "v", v, k.dtype, 4)
@@ -866,11 +883,12 @@ class KvCache:
         self.c = _KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
                           v_scale.data_ptr() if v_scale is not None else None, e, k.shape[0], k.shape[2], k.shape[1], k.shape[3],
                           k.stride(0), k.stride(1), k.stride(2), *s)
+        self._ref = C.byref(self.c)
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype, device="cuda"):
         """An empty cache (zeros) of `dtype`."""
-        import torch
+        torch = _load_torch()
         shape = (n_pages, n_kv_heads, page_size, head_dim)
         k, v = (torch.zeros(shape, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, device=device).view(dtype) for _ in range(2))
         if dtype.itemsize > 1:
@@ -879,71 +897,73 @@ class KvCache:
 
     def write(self, k, v, batch: KvBatch):
         """Rows k, v [rows, kv_heads, head_dim] (float32 or bfloat16) into the pages the batch names for them."""
-        _rows(self.device, "k", k, self.n_kv_heads, self.head_dim)
-        _rows(self.device, "v", v, self.n_kv_heads, self.head_dim)
-        if v.dtype != k.dtype or v.shape != k.shape or v.stride() != k.stride():
+        d = self.device
+        n = _rows(d, "k", k, self.n_kv_heads, self.head_dim)
+        if _rows(d, "v", v, self.n_kv_heads, self.head_dim, k.dtype) != n:
             raise ValueError("k and v have to have one type, shape and layout")
-        _call("mw_kv_write_device", self.L.mw_kv_write_device(self.device.index, _stream(self.device), C.byref(self.c), C.byref(batch._for(self.device, k.shape[0])),
-                                                              _elem(k), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)))
+        _call("mw_kv_write_device", self.L.mw_kv_write_device(d.index, _stream(d), self._ref, C.byref(batch._for(d, n[0])), _elem(k), k.data_ptr(),
+                                                              v.data_ptr(), n[1], n[2]))
 
     def read(self, batch: KvBatch, n_rows: int, dtype, out=None):
         """The batch's n_rows rows as (k, v) [rows, kv_heads, head_dim] of `dtype`; out: two tensors to fill instead of new ones
         (rows behind the last sequence are left as they are: in new ones their contents are undefined)."""
-        import torch
+        d = self.device
         if out is None:
-            k, v = (torch.empty((n_rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
+            k, v = _torch.empty((2, n_rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=d)
         else:
             k, v = out
-            _rows(self.device, "out[0]", k, self.n_kv_heads, self.head_dim)
-            _rows(self.device, "out[1]", v, self.n_kv_heads, self.head_dim)
-            if k.shape[0] != n_rows or k.dtype != dtype or v.dtype != dtype or v.shape != k.shape or v.stride() != k.stride():
-                raise ValueError("out has to be two tensors of n_rows rows in one type and layout")
-        _call("mw_kv_read_device", self.L.mw_kv_read_device(self.device.index, _stream(self.device), C.byref(self.c), C.byref(batch._for(self.device, n_rows)),
-                                                            _elem(k), k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)))
+        n = _rows(d, "out[0]", k, self.n_kv_heads, self.head_dim, dtype)
+        if _rows(d, "out[1]", v, self.n_kv_heads, self.head_dim, dtype) != n or n[0] != n_rows:
+            raise ValueError("out has to be two tensors of n_rows rows in one type and layout")
+        _call("mw_kv_read_device", self.L.mw_kv_read_device(d.index, _stream(d), self._ref, C.byref(batch._for(d, n_rows)), _elem(k), k.data_ptr(),
+                                                            v.data_ptr(), n[1], n[2]))
         return k, v
 
     def attend(self, q, batch: KvBatch, scale=None, window: int = 0, sinks: int = 0, out=None):
         """Attention of rows q [rows, heads, head_dim] (bfloat16) over their sequences' keys and values; scale defaults to
         head_dim ** -0.5.  Rows behind the last sequence are left as they are (undefined without `out`).  The workspace
         is a tensor of the current stream's, or of the graph that captures the call."""
-        import torch
-        _on(self.device, "q", q, torch.bfloat16, 3)
+        d, bf16 = self.device, _torch.bfloat16
         heads = q.shape[1]
-        _rows(self.device, "q", q, heads, self.head_dim)
+        n, qr, qh = _rows(d, "q", q, heads, self.head_dim, bf16)
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+            out = _torch.empty((n, heads, self.head_dim), dtype=bf16, device=d)
+            o_r, o_h = heads * self.head_dim, self.head_dim
         else:
-            _on(self.device, "out", out, torch.bfloat16, 3)
-            _rows(self.device, "out", out, heads, self.head_dim)
-            if out.shape[0] != q.shape[0]:
+            no, o_r, o_h = _rows(d, "out", out, heads, self.head_dim, bf16)
+            if no != n:
                 raise ValueError("out has another number of rows than q")
-        b = C.byref(batch._for(self.device, q.shape[0]))
-        need = self.L.mw_kv_attend_workspace(self.device.index, C.byref(self.c), b, heads)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _call("mw_kv_attend_device", self.L.mw_kv_attend_device(
-            self.device.index, _stream(self.device), C.byref(self.c), b, heads, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-            out.stride(1), self.head_dim ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr() if need else None, need))
+        b = C.byref(batch._for(d, n))
+        need = self.L.mw_kv_attend_workspace(d.index, self._ref, b, heads)
+        ws = _torch.empty(need, dtype=_torch.uint8, device=d) if need else None
+        rc = self.L.mw_kv_attend_device(d.index, _stream(d), self._ref, b, heads, q.data_ptr(), qr, qh, out.data_ptr(), o_r, o_h,
+                                        self.head_dim ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr() if need else None, need)
+        if rc:
+            _call("mw_kv_attend_device", rc)
         return out
 
 
 def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
     """One token per row of logits [rows, vocab] (float32 or bfloat16), drawn with u [rows] (float64, 0 <= u < 1): (ids int32,
     log probabilities float32).  temperature, top_p, min_p (float32) and top_k (int32) are per-row tensors or None."""
-    import torch
-    d, n = logits.device, logits.shape[0]
+    torch = _torch or _load_torch()
+    d = logits.device
     _on(d, "logits", logits, None, 2)
-    if logits.shape[1] > 1 and logits.stride(1) != 1:
+    n, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("the logits of a row have to be adjacent")
-    _on(d, "u", u, torch.float64, 1)
-    settings = (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32))
     if out is None:
         out = torch.empty(n, dtype=torch.int32, device=d), torch.empty(n, dtype=torch.float32, device=d)
-    for name, t, kind in (("u", u, torch.float64), *settings, ("out[0]", out[0], torch.int32), ("out[1]", out[1], torch.float32)):
-        if t is not None:
-            _on(d, name, t, kind, 1)
-            if t.shape[0] != n or not t.is_contiguous():
-                raise ValueError(f"{name} has to be contiguous with one entry per row")
-    at = [t.data_ptr() if t is not None else None for _, t, _ in settings]
-    _call("mw_sample_device", lib().mw_sample_device(d.index, _stream(d), logits.data_ptr(), _elem(logits), n, logits.shape[1], logits.stride(0), *at,
-                                                     u.data_ptr(), out[0].data_ptr(), out[1].data_ptr()))
+    f32, i32 = torch.float32, torch.int32
+    at = []
+    for name, t, kind in (("temperature", temperature, f32), ("top_k", top_k, i32), ("top_p", top_p, f32), ("min_p", min_p, f32), ("u", u, torch.float64),
+                          ("out[0]", out[0], i32), ("out[1]", out[1], f32)):
+        if t is None:
+            at.append(None)
+            continue
+        _on(d, name, t, kind, 1)
+        if t.shape[0] != n or not t.is_contiguous():
+            raise ValueError(f"{name} has to be contiguous with one entry per row")
+        at.append(t.data_ptr())
+    _call("mw_sample_device", lib().mw_sample_device(d.index, _stream(d), logits.data_ptr(), _elem(logits), n, vocab, logits.stride(0), *at))
     return out
