@@ -16,6 +16,8 @@
 // a key's scale multiplies its scores, a value's scale its probabilities, both in fp32.
 #include "decoder_ops.hpp"
 
+#include <type_traits>
+
 namespace mw {
 
 namespace {
@@ -138,23 +140,34 @@ template <int KS> __device__ __forceinline__ KeySteps key_steps(const KvView &V,
 }
 template <int KS> __device__ __forceinline__ int64_t step_key(const KeySteps &s, int i) { return i < s.n_sink ? (int64_t)i * KS : s.lo + (int64_t)(i - s.n_sink) * KS; }
 
+// The page of key j, or -1 (j is anything below 2^62; a table has at least one column where there are keys).  No branch: the
+// entry is loaded in any case, from a column that exists.
+__device__ __forceinline__ int page_of_key(const KvView &V, int seq, int64_t j, bool wanted) {
+    const int64_t col = min(max(j, (int64_t)0) >> V.shift, (int64_t)V.table_cols - 1);
+    const int page = V.table[seq * V.table_stride + col];
+    return wanted && (unsigned)page < (unsigned)V.n_pages ? page : -1;
+}
+
 // ------------------------------------------------------------------------------------------------------------------------
-// Tiles of 16 rows: four waves take every fourth step of 32 keys; no wave waits for another before the end.
+// Tiles of 16 rows: four waves take every fourth step of 32 keys; no wave waits for another before the end.  The next step's
+// rows are on their way while one is computed, their pages were looked up a step before (a key per lane).
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int RS = 32;      // keys per step
 constexpr int RW = 4;       // waves
 constexpr int VPAD = 16;    // V rows in LDS: 16 elements of padding put 8 consecutive rows on different banks for the transposing reads
 
 template <int KIND, int DH>
-__global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
+__global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
     constexpr int NS = DH / 32;        // 32-dim slices of the score product
     constexpr int ND = DH / 16;        // 16-dim tiles of the output
     constexpr int VLD = DH + VPAD;
     constexpr int EB = KIND == BF16 ? 2 : 1;
     using raw_t = typename Raw<KIND>::type;
-    __shared__ __attribute__((aligned(16))) bf16_t vt[RW][RS * VLD];
-    __shared__ float sc[RW][2 * RS];
-    __shared__ float part[RW][16][DH + 4];
+    __shared__ __attribute__((aligned(16))) union {
+        bf16_t vt[RW][RS * VLD];
+        float part[RW][16][DH + 4];
+    } U;
+    __shared__ float sc[RW][2 * RS], pw[RW][KIND == INT8 ? 1 : RS * 16];
     __shared__ float ml[RW][16][2];
     const KvView &V = A.V;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
@@ -177,66 +190,76 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
         for (int s = 0; s < NS; ++s) qf[s] = *(const u32x4 *)(qp + 32 * s);
     }
     const KeySteps ks = key_steps<RS>(V, A.window, A.sinks, p_lo, p_hi);
-    const int i0 = (int)((int64_t)ks.n * split / A.splits), i1 = (int)((int64_t)ks.n * (split + 1) / A.splits);
+    const int i0 = (int)((int64_t)ks.n * split / A.splits) + wave, i1 = (int)((int64_t)ks.n * (split + 1) / A.splits);
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    const int64_t head_off = hk * V.head_stride;
-    for (int i = i0 + wave; i < i1; i += RW) {
-        const int64_t key0 = step_key<RS>(ks, i);
-        // lane -> key fr of tile 0 and of tile 1: its page; keys no row sees are not loaded
-        raw_t kr[2][NS], vr[2][NS];
-        bool dead[2];
-        int64_t off[2];
+    const char *kbase = V.k + (hk * V.head_stride + 8 * g) * EB, *vbase = V.v + (hk * V.head_stride + 8 * g) * EB;
+    const float *sbase = (lane < RS ? V.ks : V.vs) + hk * V.s_head;
+    struct Step {
+        raw_t k[2][NS], v[2][NS];
+        float scale;
+        unsigned dead;  // keys that no row sees, a bit each
+    };
+    // page of key lane & 31 of step i
+    auto page_of = [&](int i) {
+        const int64_t j = step_key<RS>(ks, i) + (lane & 31);
+        return page_of_key(V, seq, j, i < i1 && j < ks.hi && !(A.window > 0 && j <= p_lo - A.window && j >= A.sinks));
+    };
+    // (rows that are not there come from page 0 and are dropped later)
+    auto load = [&](Step &x, int i, int page) {
+        const int64_t j = step_key<RS>(ks, i) + (lane & 31);
+        const int pg = max(page, 0), r = (int)j & V.mask;
+        const int64_t off = (pg * V.page_stride + r * V.row_stride) * EB;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int64_t j = key0 + 16 * t + fr;
-            const int page = j < ks.hi ? kv_page(V, seq, j) : -1;
-            dead[t] = page < 0 || (A.window > 0 && j <= p_lo - A.window && j >= A.sinks);
-            off[t] = dead[t] ? head_off : page * V.page_stride + head_off + (j & V.mask) * V.row_stride;
+            const int64_t at = __shfl(off, 16 * t + fr);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                kr[t][s] = *(const raw_t *)(V.k + (off[t] + 32 * s + 8 * g) * EB);
-                vr[t][s] = *(const raw_t *)(V.v + (off[t] + 32 * s + 8 * g) * EB);
-            }
-            if constexpr (KIND != BF16) {
-                // lanes 0 .. 15 fetch the key's scale, 16 .. 31 the value's
-                if (g < 2) {
-                    const float *sp = g ? V.vs : V.ks;
-                    const int64_t so = dead[t] ? hk * V.s_head : page * V.s_page + hk * V.s_head + (j & V.mask) * V.s_row;
-                    sc[wave][g * RS + 16 * t + fr] = sp[so];
-                }
+                x.k[t][s] = *(const raw_t *)(kbase + at + 32 * s * EB);
+                x.v[t][s] = *(const raw_t *)(vbase + at + 32 * s * EB);
             }
         }
+        if constexpr (KIND != BF16) x.scale = sbase[pg * V.s_page + r * V.s_row];  // lanes 0 .. 31 the keys', the others the values'
+        x.dead = (unsigned)__ballot(page < 0);
+    };
+    auto step = [&](Step &x, int i) {
+        const int64_t key0 = step_key<RS>(ks, i);
+        if constexpr (KIND != BF16) sc[wave][lane] = x.scale;
         // V rows -> LDS (dead ones as zeros)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            const bool gone = (x.dead >> (16 * t + fr)) & 1;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                u32x4 x = to_bf16<KIND>(vr[t][s]);
-                if (dead[t]) x = u32x4{0, 0, 0, 0};
-                *(u32x4 *)&vt[wave][(16 * t + fr) * VLD + 32 * s + 8 * g] = x;
+            for (int c = 0; c < NS; ++c) {
+                u32x4 y = to_bf16<KIND>(x.v[t][c]);
+                if (x.dead != 0) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) y[q] = gone ? 0 : y[q];
+                }
+                *(u32x4 *)&U.vt[wave][(16 * t + fr) * VLD + 32 * c + 8 * g] = y;
             }
+        }
         __builtin_amdgcn_wave_barrier();  // what other lanes of the wave read below is written above (LDS keeps a wave's order)
-        // scores
+        // scores (taken out of the result vectors at once: an element set under a branch there was compiled wrongly)
         float s[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NS; ++c)
-                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, to_bf16<KIND>(kr[t][c])), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, to_bf16<KIND>(x.k[t][c])), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = a[r] * (KIND == BF16 ? A.c : sc[wave][16 * t + 4 * g + r] * A.c);
         }
         // the 32 keys this lane's row sees, a bit each
-        unsigned vis = ~(unsigned)(__ballot(dead[0]) & 0xffff) & ~((unsigned)(__ballot(dead[1]) & 0xffff) << 16);
-        vis &= low_bits(p - key0 + 1);
-        if (A.window > 0) vis &= ~low_bits(p - A.window - key0 + 1) | low_bits((int64_t)A.sinks - key0);
-        const bool whole = __ballot(vis != ~0u) == 0;
-        const unsigned mine = vis >> (4 * g);  // bit 16 t + r: the lane's key r of tile t
+        unsigned vis = ~0u;
+        const bool whole = x.dead == 0 && key0 + RS - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + RS <= A.sinks);
         if (!whole) {
+            vis = ~x.dead & low_bits(p - key0 + 1);
+            if (A.window > 0) vis &= ~low_bits(p - A.window - key0 + 1) | low_bits((int64_t)A.sinks - key0);
+            const unsigned mine = vis >> (4 * g);  // bit 16 t + r: the lane's key r of tile t
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -262,7 +285,7 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
                 ps += e;
                 // (the scale of a value that is not seen may be anything)
                 if constexpr (KIND == BF16) pv[t][r] = e;
-                else pv[t][r] = mine & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
+                else pv[t][r] = (vis >> (4 * g)) & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
             }
         l = l * corr + ps;
 #pragma unroll
@@ -273,13 +296,14 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int c = 0; c < NS; ++c) bad |= !dead[t] && has_nonfinite(to_bf16<KIND>(vr[t][c]));
+                for (int c = 0; c < NS; ++c) bad |= !((x.dead >> (16 * t + fr)) & 1) && has_nonfinite(to_bf16<KIND>(x.v[t][c]));
             per_key = __ballot(bad) != 0;
         }
         if (!per_key) {
+            // the residue of the probabilities' rounding goes through a second product: these kernels wait for memory, not for the MFMAs
             const u32x4 pb = {pack_bf16(pv[0][0], pv[0][1]), pack_bf16(pv[0][2], pv[0][3]), pack_bf16(pv[1][0], pv[1][1]), pack_bf16(pv[1][2], pv[1][3])};
             const u32x4 pl = low_part(&pv[0][0], pb);
-            const bf16_t *vb = &vt[wave][(4 * g + (fr >> 2)) * VLD + (fr & 3) * 4];
+            const bf16_t *vb = &U.vt[wave][(4 * g + (fr >> 2)) * VLD + (fr & 3) * 4];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * d)));
@@ -288,27 +312,42 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
             }
-        } else {  // key by key, rows that see it only (part is free until the end)
+        } else {  // key by key, rows that see it only
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) (&part[wave][0][0])[(16 * t + 4 * g + r) * 16 + fr] = pv[t][r];
+                for (int r = 0; r < 4; ++r) pw[wave][(16 * t + 4 * g + r) * 16 + fr] = pv[t][r];
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
             for (int k = 0; k < RS; ++k) {
-                const float pk = (&part[wave][0][0])[k * 16 + fr];
-                const bf16_t *vrow = &vt[wave][k * VLD + 4 * g];
+                const float pk = pw[wave][k * 16 + fr];
+                const bf16_t *vrow = &U.vt[wave][k * VLD + 4 * g];
                 const bool ok = (vis >> k) & 1;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = fmaf(pk, __uint_as_float((unsigned)vrow[16 * d + e] << 16), o[d][e]);
-                        o[d][e] = ok ? x : o[d][e];
+                        const float y = fmaf(pk, __uint_as_float((unsigned)vrow[16 * d + e] << 16), o[d][e]);
+                        o[d][e] = ok ? y : o[d][e];
                     }
             }
         }
         __builtin_amdgcn_wave_barrier();  // the next step's rows come after this one's reads
+    };
+    if (i0 < i1) {
+        Step x, y;
+        int page = page_of(i0);
+        load(x, i0, page);
+        page = page_of(i0 + RW);
+        for (int i = i0; i < i1; i += 2 * RW) {
+            load(y, min(i + RW, i1 - 1), page);
+            page = page_of(i + 2 * RW);
+            step(x, i);
+            if (i + RW >= i1) break;
+            load(x, min(i + 2 * RW, i1 - 1), page);
+            page = page_of(i + 3 * RW);
+            step(y, i + RW);
+        }
     }
     l = xor_sum<32>(xor_sum<16>(l));
     // join the four waves
@@ -323,7 +362,7 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
     const float ref = M == -INFINITY ? 0.0f : M;
     const float f = __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *(f32x4 *)&part[wave][fr][16 * d + 4 * g] = o[d] * f;
+    for (int d = 0; d < ND; ++d) *(f32x4 *)&U.part[wave][fr][16 * d + 4 * g] = o[d] * f;
     __syncthreads();
     // 256 threads: row threadIdx / 16, DH / 16 dims each
     constexpr int E = DH / 16;
@@ -338,7 +377,7 @@ __global__ __launch_bounds__(64 * RW) void attend_rows_kernel(AttendP A) {
     for (int w = 0; w < RW; ++w) {
         L += ml[w][r][1] * __builtin_amdgcn_exp2f(ml[w][r][0] - rr);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += part[w][r][d0 + e];
+        for (int e = 0; e < E; ++e) acc[e] += U.part[w][r][d0 + e];
     }
     const int rw = first + r, tk = rw / A.group, hd = hk * A.group + rw % A.group;
     if (A.splits == 1) {
@@ -390,7 +429,6 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
     const int tok = row / A.group, head = hk * A.group + row % A.group;
     const int64_t p = p_base + tok;
     const int64_t p_lo = p_base + first / A.group, p_hi = p_base + (first + n_tile - 1) / A.group;
-    const bool active = wave * 32 < n_tile;
     u32x4 qf[DH / 16];
     {
         const bf16_t *qp = A.q + (row0 + tok) * A.q_row + head * A.q_head + 8 * h;
@@ -408,41 +446,41 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
     const int srow = tid / LPR, sub = tid % LPR;
     // page of key `lane` of step i, -1 when no row of the tile can see it
     auto page_of = [&](int i) -> int {
-        if (i >= i1) return -1;
         const int64_t j = step_key<CK>(ks, i) + lane;
-        if (j >= ks.hi || (A.window > 0 && j <= p_lo - A.window && j >= A.sinks)) return -1;
-        return kv_page(V, seq, j);
+        return page_of_key(V, seq, j, i < i1 && j < ks.hi && !(A.window > 0 && j <= p_lo - A.window && j >= A.sinks));
     };
     // whether every row of the tile sees every key of the step at key0 (pages apart)
     auto all_see = [&](int64_t key0) { return key0 + CK - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + CK <= A.sinks); };
     raw_t rk[NP], rv[NP];
     float rs = 0.0f;
-    unsigned rdead = 0;  // passes whose row is not there
+    const char *kbase = V.k + (hk * V.head_stride + sub * 8) * EB, *vbase = V.v + (hk * V.head_stride + sub * 8) * EB;
+    const float *sbase = (wave ? V.vs : V.ks) + hk * V.s_head;
+    // (rows that are not there come from page 0 and are dropped when they are stored)
     auto load = [&](int64_t key0, int page) {
-        rdead = 0;
+        const int pg = max(page, 0), j = (int)(key0 + lane) & V.mask;
+        const int64_t off = (pg * V.page_stride + j * V.row_stride) * EB;
 #pragma unroll
         for (int s = 0; s < NP; ++s) {
-            const int r = s * RPP + srow, pg = __shfl(page, r);
-            rdead |= (pg < 0) << s;
-            const int64_t off = (pg < 0 ? 0 : pg * V.page_stride + ((key0 + r) & V.mask) * V.row_stride) + hk * V.head_stride + sub * 8;
-            rk[s] = *(const raw_t *)(V.k + off * EB);
-            rv[s] = *(const raw_t *)(V.v + off * EB);
+            const int64_t at = __shfl(off, s * RPP + srow);
+            rk[s] = *(const raw_t *)(kbase + at);
+            rv[s] = *(const raw_t *)(vbase + at);
         }
         if constexpr (KIND != BF16) {  // waves 0 and 1: the keys' and the values' scales, a key per lane
-            if (wave < 2) {
-                const int64_t so = (page < 0 ? 0 : page * V.s_page + ((key0 + lane) & V.mask) * V.s_row) + hk * V.s_head;
-                rs = (wave ? V.vs : V.ks)[so];
-            }
+            if (wave < 2) rs = sbase[pg * V.s_page + j * V.s_row];
         }
     };
-    auto store = [&](int buf, bool check) {
+    auto store = [&](int buf, bool check, unsigned long long gone) {
         bool bad = false;
 #pragma unroll
         for (int s = 0; s < NP; ++s) {
             const int r = s * RPP + srow;
             *(u32x4 *)&kt[buf][r * KLD + sub * 8] = to_bf16<KIND>(rk[s]);
             u32x4 x = to_bf16<KIND>(rv[s]);
-            if ((rdead >> s) & 1) x = u32x4{0, 0, 0, 0};
+            if (gone != 0) {
+                const bool out = (gone >> r) & 1;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[q] = out ? 0 : x[q];
+            }
             if (KIND != INT8 && check) bad |= has_nonfinite(x);
             *(u32x4 *)&vt[buf][r * VLD + sub * 8] = x;
         }
@@ -459,151 +497,164 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
         const int64_t key0 = step_key<CK>(ks, i0);
         load(key0, page_n);
         page_n = page_of(i0 + 1);
-        store(0, !all_see(key0));
+        store(0, !all_see(key0), dead);
     }
     __syncthreads();
-    for (int i = i0; i < i1; ++i) {
-        const int cur = (i - i0) & 1;
-        const int64_t key0 = step_key<CK>(ks, i);
-        const bool more = i + 1 < i1;
-        if (more) {
-            dead_n = __ballot(page_n < 0);
-            load(step_key<CK>(ks, i + 1), page_n);
-            page_n = page_of(i + 2);
+    // one step; MASKED: some row may not see some key of it
+    auto step = [&](auto masked, int cur, int64_t key0) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const bf16_t *kb = kt[cur], *vb = vt[cur];
+        float s[2][16];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 a;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) a[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < DH / 16; ++c) {
+                const u32x4 kf = *(const u32x4 *)(kb + (32 * t + fr) * KLD + 16 * c + 8 * h);
+                a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[t][r] = a[r];
         }
-        const bool clear = dead == 0 && all_see(key0);
-        if (active) {
-            const bf16_t *kb = kt[cur], *vb = vt[cur];
-            float s[2][16];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x16 a;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) a[r] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < DH / 16; ++c) {
-                    const u32x4 kf = *(const u32x4 *)(kb + (32 * t + fr) * KLD + 16 * c + 8 * h);
-                    a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[t][r] = a[r];
-            }
-            if constexpr (KIND != BF16) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const f32x4 f = *(const f32x4 *)&sc[cur][0][32 * t + 8 * b + 4 * h];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
-                    }
-            }
-            unsigned vis[2] = {~0u, ~0u};
-            if (!clear) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    unsigned v = ~(unsigned)(dead >> (32 * t)) & low_bits(p - key0 + 1 - 32 * t);
-                    if (A.window > 0) v &= ~low_bits(p - A.window - key0 + 1 - 32 * t) | low_bits((int64_t)A.sinks - key0 - 32 * t);
-                    vis[t] = v;
-                    const unsigned mine = v >> (4 * h);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[t][r] = mine & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : -INFINITY;
-                }
-            }
-            // running maximum (of the unscaled scores; the scale rides in the exponent's fma)
-            float mx = s[0][0];
+        if constexpr (KIND != BF16) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-            mx = xor_max<32>(mx);
-            if (__ballot(mx > m)) {
-                const float nm = fmaxf(mx, m), ref = nm == -INFINITY ? 0.0f : nm;
-                const float corr = __builtin_amdgcn_exp2f((m - ref) * A.c);
-                m = nm;
-                l *= corr;
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4 f = *(const f32x4 *)&sc[cur][0][32 * t + 8 * b + 4 * h];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
+                }
+        }
+        unsigned vis[2] = {~0u, ~0u};
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                unsigned v = ~(unsigned)(dead >> (32 * t)) & low_bits(p - key0 + 1 - 32 * t);
+                if (A.window > 0) v &= ~low_bits(p - A.window - key0 + 1 - 32 * t) | low_bits((int64_t)A.sinks - key0 - 32 * t);
+                vis[t] = v;
+                const unsigned mine = v >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][r] = mine & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : -INFINITY;
+            }
+        }
+        // running maximum (of the unscaled scores; the scale rides in the exponent's fma)
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+        mx = xor_max<32>(mx);
+        // the reference follows the maximum only when that has left it by more than 2^8 (probabilities stay below 256, their
+        // relative roundings are the same): rescaling the result at every new maximum of one of 32 rows cost a quarter of a step
+        if (__ballot((mx - m) * A.c > 8.0f || (m == -INFINITY && mx > m))) {
+            const float nm = fmaxf(mx, m), base = nm == -INFINITY ? 0.0f : nm;
+            const float corr = __builtin_amdgcn_exp2f((m - base) * A.c);
+            m = nm;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= corr;
+        }
+        const float ref = m == -INFINITY ? 0.0f : -m * A.c;
+        float ps = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], A.c, ref));
+                ps += s[t][r];
+            }
+        l += ps;
+        if constexpr (KIND != BF16) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4 f = *(const f32x4 *)&sc[cur][1][32 * t + 8 * b + 4 * h];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
+                }
+            if (MASKED) {  // (the scale of a value that is not seen may be anything)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[t][r] = (vis[t] >> (4 * h)) & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : 0.0f;
+            }
+        }
+        if (KIND == INT8 || !MASKED || odd[cur] == 0) {
+            const int gi = lane >> 4, ii = lane & 15;
+            const bf16_t *va = vb + (4 * h + (ii >> 2)) * VLD + 16 * (gi & 1) + (ii & 3) * 4;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float *e = &s[c >> 1][8 * (c & 1)];
+                const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
+                u32x4 pl = {0, 0, 0, 0};
+                if constexpr (KIND == INT8) pl = low_part(e, pb);
+#pragma unroll
+                for (int d = 0; d < DH / 32; ++d) {
+                    const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + 16 * c * VLD + 32 * d)));
+                    const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + (16 * c + 8) * VLD + 32 * d)));
+                    const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+                    if constexpr (KIND == INT8)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
+                }
+            }
+        } else {
+            // values that are not finite and that some rows do not see (0 x inf = NaN): key by key, rows that see it only
+#pragma unroll 1
+            for (int k = 0; k < CK; ++k) {
+                const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the 32 of its half
+                float mine = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
+                const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
+                const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
+                const bf16_t *vrow = vb + k * VLD + 4 * h;
 #pragma unroll
                 for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] *= corr;
-            }
-            const float ref = m == -INFINITY ? 0.0f : -m * A.c;
-            float ps = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], A.c, ref));
-                    ps += s[t][r];
-                }
-            l += ps;
-            if constexpr (KIND != BF16) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const f32x4 f = *(const f32x4 *)&sc[cur][1][32 * t + 8 * b + 4 * h];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
+                    for (int q = 0; q < 16; ++q) {
+                        const float x = fmaf(pk, __uint_as_float((unsigned)vrow[32 * d + 8 * (q >> 2) + (q & 3)] << 16), o[d][q]);
+                        o[d][q] = ok ? x : o[d][q];
                     }
-                if (!clear) {  // (the scale of a value that is not seen may be anything)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[t][r] = (vis[t] >> (4 * h)) & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : 0.0f;
-                }
-            }
-            if (KIND == INT8 || clear || odd[cur] == 0) {
-                const int gi = lane >> 4, ii = lane & 15;
-                const bf16_t *va = vb + (4 * h + (ii >> 2)) * VLD + 16 * (gi & 1) + (ii & 3) * 4;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float *e = &s[c >> 1][8 * (c & 1)];
-                    const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
-                    u32x4 pl = {0, 0, 0, 0};
-                    if constexpr (KIND == INT8) pl = low_part(e, pb);
-#pragma unroll
-                    for (int d = 0; d < DH / 32; ++d) {
-                        const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + 16 * c * VLD + 32 * d)));
-                        const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + (16 * c + 8) * VLD + 32 * d)));
-                        const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
-                        if constexpr (KIND == INT8)
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
-                    }
-                }
-            } else {
-                // values that are not finite and that some rows do not see (0 x inf = NaN): key by key, rows that see it only
-#pragma unroll 1
-                for (int k = 0; k < CK; ++k) {
-                    const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the 32 of its half
-                    float mine = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
-                    const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
-                    const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
-                    const bf16_t *vrow = vb + k * VLD + 4 * h;
-#pragma unroll
-                    for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            const float x = fmaf(pk, __uint_as_float((unsigned)vrow[32 * d + 8 * (q >> 2) + (q & 3)] << 16), o[d][q]);
-                            o[d][q] = ok ? x : o[d][q];
-                        }
-                }
             }
         }
-        if (more) {
-            // (the other buffer was last read before the previous barrier)
-            if (KIND != INT8 && tid == 0) odd[cur ^ 1] = 0;
-            if (KIND != INT8 && !all_see(step_key<CK>(ks, i + 1))) __syncthreads();
-            store(cur ^ 1, !all_see(step_key<CK>(ks, i + 1)));
+    };
+    int i = i0, cur = 0;
+    // the next step's loads, this one, the next one's rows into the other buffer (last read before the previous barrier)
+    auto advance = [&](auto masked) {
+        const int64_t key0 = step_key<CK>(ks, i);
+        const bool more = i + 1 < i1;
+        dead_n = __ballot(page_n < 0);
+        load(step_key<CK>(ks, more ? i + 1 : i), page_n);  // (behind the last step: loaded, not used)
+        page_n = page_of(i + 2);
+        step(masked, cur, key0);
+        const bool check = more && !all_see(step_key<CK>(ks, i + 1));
+        if (KIND != INT8) {
+            if (check) {
+                if (tid == 0) odd[cur ^ 1] = 0;
+                __syncthreads();
+            }
         }
+        store(cur ^ 1, check, dead_n);
         dead = dead_n;
+        cur ^= 1;
+        ++i;
         __syncthreads();
+    };
+    // steps that every row sees whole run in a loop of their own: with the masks' code in it the compiler kept two copies of the
+    // result and spilled
+    while (i < i1) {
+        while (i < i1 && dead == 0 && all_see(step_key<CK>(ks, i))) advance(std::false_type{});
+        if (i < i1) advance(std::true_type{});
     }
     l += __shfl_xor(l, 32);
-    if (!active || wave * 32 + fr >= n_tile) return;
+    if (wave * 32 + fr >= n_tile) return;
     const bool part = A.splits > 1;
     const float inv = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t at = ((int64_t)split * V.n_rows + row0 + tok) * A.n_heads + head;
