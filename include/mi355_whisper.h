@@ -156,8 +156,9 @@ int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache,
    value head h / (n_heads / n_kv_heads).  q and out: bf16, head h of row t at t * stride + h * head_stride, 16-byte aligned.
    Scores, softmax and sums in fp32; the probabilities are rounded to bf16 for the product with v.  A row that sees nothing
    is zero.  Invisible keys and values are never used, whatever they hold.  scale > 0, finite.  workspace: at least
-   mw_kv_attend_workspace bytes for the same device, cache, batch and n_heads (may be 0 bytes), 16-byte aligned. */
-size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads);
+   mw_kv_attend_workspace bytes for the same device, cache, batch, n_heads, window and sinks (may be 0 bytes), 16-byte aligned. */
+size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads, int window,
+                              int sinks);
 int mw_kv_attend_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads,
                         const void *q, int64_t q_row_stride, int64_t q_head_stride, void *out, int64_t out_row_stride,
                         int64_t out_head_stride, float scale, int window, int sinks, void *workspace, size_t workspace_bytes);

@@ -229,7 +229,7 @@ def lib():
     L.mw_kv_write_device.argtypes = [C.c_int, P, KC, KB, C.c_int, P, P, I64, I64]
     L.mw_kv_read_device.argtypes = [C.c_int, P, KC, KB, C.c_int, P, P, I64, I64]
     L.mw_kv_attend_workspace.restype = C.c_size_t
-    L.mw_kv_attend_workspace.argtypes = [C.c_int, KC, KB, C.c_int]
+    L.mw_kv_attend_workspace.argtypes = [C.c_int, KC, KB, C.c_int, C.c_int, C.c_int]
     L.mw_kv_attend_device.argtypes = [C.c_int, P, KC, KB, C.c_int, P, I64, I64, P, I64, I64, C.c_float, C.c_int, C.c_int, P, C.c_size_t]
     L.mw_sample_device.argtypes = [C.c_int, P, P, C.c_int, C.c_int, C.c_int, I64, P, P, P, P, P, P, P]
     L.mw_mel_n_len.argtypes = [P]
@@ -934,7 +934,7 @@ class KvCache:
             if no != n:
                 raise ValueError("out has another number of rows than q")
         b = C.byref(batch._for(d, n))
-        need = self.L.mw_kv_attend_workspace(d.index, self._ref, b, heads)
+        need = self.L.mw_kv_attend_workspace(d.index, self._ref, b, heads, window, sinks)
         ws = _torch.empty(need, dtype=_torch.uint8, device=d) if need else None
         rc = self.L.mw_kv_attend_device(d.index, _stream(d), self._ref, b, heads, q.data_ptr(), qr, qh, out.data_ptr(), o_r, o_h,
                                         self.head_dim ** -0.5 if scale is None else scale, window, sinks, ws.data_ptr() if need else None, need)

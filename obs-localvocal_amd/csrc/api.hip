@@ -882,11 +882,12 @@ int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache,
         return 0;
     });
 }
-size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads) {
+size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads,
+                              int window, int sinks) {
     size_t need = 0;
     if (!cache || !batch) return 0;
     (void)guarded("mw_kv_attend_workspace", [&]() {
-        need = kv_attend_workspace(compute_units(device), *cache, *batch, n_heads);
+        need = kv_attend_workspace(compute_units(device), *cache, *batch, n_heads, window, sinks);
         return 0;
     });
     return need;  // refused arguments: 0, and the call itself says why

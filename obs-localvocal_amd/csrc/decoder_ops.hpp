@@ -22,7 +22,7 @@ struct KvAttendArgs {
     void *ws = nullptr;
     size_t ws_bytes = 0;
 };
-size_t kv_attend_workspace(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads);
+size_t kv_attend_workspace(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, int window, int sinks);
 void launch_kv_attend(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendArgs &a, hipStream_t st);
 struct SampleArgs {
     const void *logits = nullptr;

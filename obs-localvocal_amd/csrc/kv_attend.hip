@@ -41,7 +41,7 @@ struct AttendP {
     bf16_t *out;
     int64_t o_row, o_head;
     float c;  // scale log2(e)
-    int window, sinks, splits, tiles;
+    int window, sinks, splits, split_steps, tiles;
     float *ws_o, *ws_ml;  // [splits][n_rows][n_heads][head_dim], [splits][n_rows][n_heads][2]
 };
 
@@ -49,6 +49,15 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
+// signed byte B of w as a float, in one instruction (from C every other one came with a v_bfe_i32 of its own)
+template <int B> __device__ __forceinline__ float byte_of(unsigned w) {
+    float f;
+    if constexpr (B == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+    else if constexpr (B == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+    else if constexpr (B == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+    else asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+    return f;
+}
 // 8 cache elements -> 8 bf16
 template <int KIND> struct Raw { using type = u32x2; };
 template <> struct Raw<BF16> { using type = u32x4; };
@@ -61,15 +70,16 @@ template <int KIND> __device__ __forceinline__ u32x4 to_bf16(typename Raw<KIND>:
                      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.y, 1.0f, false)),
                      __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.y, 1.0f, true))};
     } else {
-        u32x4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned w = i < 2 ? r.x : r.y;
-            const int s = (i & 1) * 16;
-            o[i] = pack_bf16((float)(signed char)(w >> s), (float)(signed char)(w >> (s + 8)));
-        }
-        return o;
+        return u32x4{pack_bf16(byte_of<0>(r.x), byte_of<1>(r.x)), pack_bf16(byte_of<2>(r.x), byte_of<3>(r.x)),
+                     pack_bf16(byte_of<0>(r.y), byte_of<1>(r.y)), pack_bf16(byte_of<2>(r.y), byte_of<3>(r.y))};
     }
+}
+// fragment f (8 elements) of 16 bytes of a row: all of it in bf16, one of two in 8 bits.  The order in which a lane has the dims
+// is free as long as the queries' fragments have the same: 16 bytes a lane are 64 adjacent bytes of a row (with 8, an 8-bit
+// cache was read in pieces of 32 and twice as many loads).
+template <int KIND> __device__ __forceinline__ u32x4 fragment(u32x4 x, int f) {
+    if constexpr (KIND == BF16) return x;
+    else return to_bf16<KIND>(f ? u32x2{x.z, x.w} : u32x2{x.x, x.y});
 }
 // what the rounding of 8 probabilities to bf16 (hi) left, itself in bf16
 __device__ __forceinline__ u32x4 low_part(const float *e, u32x4 hi) {
@@ -140,6 +150,16 @@ template <int KS> __device__ __forceinline__ KeySteps key_steps(const KvView &V,
 }
 template <int KS> __device__ __forceinline__ int64_t step_key(const KeySteps &s, int i) { return i < s.n_sink ? (int64_t)i * KS : s.lo + (int64_t)(i - s.n_sink) * KS; }
 
+// The steps of a split: all splits but a sequence's last have the same number, so that long and short sequences of a batch give
+// workgroups of one size; the last split takes what the expected lengths did not foresee.
+struct KeyRange {
+    int begin, end;
+};
+__device__ __forceinline__ KeyRange split_steps(int n, int split, const AttendP &A) {
+    const int64_t b = (int64_t)split * A.split_steps, e = b + A.split_steps;
+    return {(int)min(b, (int64_t)n), split == A.splits - 1 ? n : (int)min(e, (int64_t)n)};
+}
+
 // The page of key j, or -1 (j is anything below 2^62; a table has at least one column where there are keys).  No branch: the
 // entry is loaded in any case, from a column that exists.
 __device__ __forceinline__ int page_of_key(const KvView &V, int seq, int64_t j, bool wanted) {
@@ -162,7 +182,8 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
     constexpr int ND = DH / 16;        // 16-dim tiles of the output
     constexpr int VLD = DH + VPAD;
     constexpr int EB = KIND == BF16 ? 2 : 1;
-    using raw_t = typename Raw<KIND>::type;
+    constexpr int NL = DH * EB / 64;   // 16-byte loads of a lane per row
+    constexpr int FL = NS / NL;        // fragments (8 elements) in each
     __shared__ __attribute__((aligned(16))) union {
         bf16_t vt[RW][RS * VLD];
         float part[RW][16][DH + 4];
@@ -185,20 +206,21 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
     const int64_t p_lo = p_base + first / A.group, p_hi = p_base + (first + n_tile - 1) / A.group;
     u32x4 qf[NS];
     {
-        const bf16_t *qp = A.q + (row0 + tok) * A.q_row + head * A.q_head + 8 * g;
+        const bf16_t *qp = A.q + (row0 + tok) * A.q_row + head * A.q_head + 8 * FL * g;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) qf[s] = *(const u32x4 *)(qp + 32 * s);
+        for (int s = 0; s < NS; ++s) qf[s] = *(const u32x4 *)(qp + s / FL * 32 * FL + 8 * (s % FL));
     }
     const KeySteps ks = key_steps<RS>(V, A.window, A.sinks, p_lo, p_hi);
-    const int i0 = (int)((int64_t)ks.n * split / A.splits) + wave, i1 = (int)((int64_t)ks.n * (split + 1) / A.splits);
+    const KeyRange range = split_steps(ks.n, split, A);
+    const int i0 = range.begin + wave, i1 = range.end;
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    const char *kbase = V.k + (hk * V.head_stride + 8 * g) * EB, *vbase = V.v + (hk * V.head_stride + 8 * g) * EB;
+    const char *kbase = V.k + hk * V.head_stride * EB + 16 * g, *vbase = V.v + hk * V.head_stride * EB + 16 * g;
     const float *sbase = (lane < RS ? V.ks : V.vs) + hk * V.s_head;
     struct Step {
-        raw_t k[2][NS], v[2][NS];
+        u32x4 k[2][NL], v[2][NL];
         float scale;
         unsigned dead;  // keys that no row sees, a bit each
     };
@@ -216,29 +238,30 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
         for (int t = 0; t < 2; ++t) {
             const int64_t at = __shfl(off, 16 * t + fr);
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                x.k[t][s] = *(const raw_t *)(kbase + at + 32 * s * EB);
-                x.v[t][s] = *(const raw_t *)(vbase + at + 32 * s * EB);
+            for (int s = 0; s < NL; ++s) {
+                x.k[t][s] = *(const u32x4 *)(kbase + at + 64 * s);
+                x.v[t][s] = *(const u32x4 *)(vbase + at + 64 * s);
             }
         }
         if constexpr (KIND != BF16) x.scale = sbase[pg * V.s_page + r * V.s_row];  // lanes 0 .. 31 the keys', the others the values'
         x.dead = (unsigned)__ballot(page < 0);
     };
-    auto step = [&](Step &x, int i) {
-        const int64_t key0 = step_key<RS>(ks, i);
+    // one step; MASKED: some row may not see some key of it
+    auto step = [&](auto masked, Step &x, int64_t key0) {
+        constexpr bool MASKED = decltype(masked)::value;
         if constexpr (KIND != BF16) sc[wave][lane] = x.scale;
         // V rows -> LDS (dead ones as zeros)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const bool gone = (x.dead >> (16 * t + fr)) & 1;
+            const bool gone = MASKED && (x.dead >> (16 * t + fr)) & 1;
 #pragma unroll
             for (int c = 0; c < NS; ++c) {
-                u32x4 y = to_bf16<KIND>(x.v[t][c]);
-                if (x.dead != 0) {
+                u32x4 y = fragment<KIND>(x.v[t][c / FL], c % FL);
+                if constexpr (MASKED) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) y[q] = gone ? 0 : y[q];
                 }
-                *(u32x4 *)&U.vt[wave][(16 * t + fr) * VLD + 32 * c + 8 * g] = y;
+                *(u32x4 *)&U.vt[wave][(16 * t + fr) * VLD + c / FL * 32 * FL + 8 * FL * g + 8 * (c % FL)] = y;
             }
         }
         __builtin_amdgcn_wave_barrier();  // what other lanes of the wave read below is written above (LDS keeps a wave's order)
@@ -249,14 +272,13 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
             f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NS; ++c)
-                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, to_bf16<KIND>(x.k[t][c])), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fragment<KIND>(x.k[t][c / FL], c % FL)), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = a[r] * (KIND == BF16 ? A.c : sc[wave][16 * t + 4 * g + r] * A.c);
         }
         // the 32 keys this lane's row sees, a bit each
         unsigned vis = ~0u;
-        const bool whole = x.dead == 0 && key0 + RS - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + RS <= A.sinks);
-        if (!whole) {
+        if constexpr (MASKED) {
             vis = ~x.dead & low_bits(p - key0 + 1);
             if (A.window > 0) vis &= ~low_bits(p - A.window - key0 + 1) | low_bits((int64_t)A.sinks - key0);
             const unsigned mine = vis >> (4 * g);  // bit 16 t + r: the lane's key r of tile t
@@ -285,18 +307,18 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
                 ps += e;
                 // (the scale of a value that is not seen may be anything)
                 if constexpr (KIND == BF16) pv[t][r] = e;
-                else pv[t][r] = (vis >> (4 * g)) & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
+                else pv[t][r] = !MASKED || (vis >> (4 * g)) & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
             }
         l = l * corr + ps;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= corr;
         bool per_key = false;
-        if (KIND != INT8 && !whole) {  // a value that some rows see and others do not must not reach the others: 0 x inf = NaN
+        if constexpr (KIND != INT8 && MASKED) {  // a value that some rows see and others do not must not reach the others: 0 x inf = NaN
             bool bad = false;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int c = 0; c < NS; ++c) bad |= !((x.dead >> (16 * t + fr)) & 1) && has_nonfinite(to_bf16<KIND>(x.v[t][c]));
+                for (int c = 0; c < NS; ++c) bad |= !((x.dead >> (16 * t + fr)) & 1) && has_nonfinite(fragment<KIND>(x.v[t][c / FL], c % FL));
             per_key = __ballot(bad) != 0;
         }
         if (!per_key) {
@@ -334,6 +356,12 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
         }
         __builtin_amdgcn_wave_barrier();  // the next step's rows come after this one's reads
     };
+    auto run = [&](Step &x, int i) {
+        const int64_t key0 = step_key<RS>(ks, i);
+        const bool whole = x.dead == 0 && key0 + RS - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + RS <= A.sinks);
+        if (whole) step(std::false_type{}, x, key0);
+        else step(std::true_type{}, x, key0);
+    };
     if (i0 < i1) {
         Step x, y;
         int page = page_of(i0);
@@ -342,11 +370,11 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
         for (int i = i0; i < i1; i += 2 * RW) {
             load(y, min(i + RW, i1 - 1), page);
             page = page_of(i + 2 * RW);
-            step(x, i);
+            run(x, i);
             if (i + RW >= i1) break;
             load(x, min(i + 2 * RW, i1 - 1), page);
             page = page_of(i + 3 * RW);
-            step(y, i + RW);
+            run(y, i + RW);
         }
     }
     l = xor_sum<32>(xor_sum<16>(l));
@@ -436,7 +464,8 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
         for (int s = 0; s < DH / 16; ++s) qf[s] = *(const u32x4 *)(qp + 16 * s);
     }
     const KeySteps ks = key_steps<CK>(V, A.window, A.sinks, p_lo, p_hi);
-    const int i0 = (int)((int64_t)ks.n * split / A.splits), i1 = (int)((int64_t)ks.n * (split + 1) / A.splits);
+    const KeyRange range = split_steps(ks.n, split, A);
+    const int i0 = range.begin, i1 = range.end;
     f32x16 o[DH / 32];
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d)
@@ -707,21 +736,24 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendP A) {
 struct Plan {
     int rows;  // of a tile
     int64_t tiles;
-    int splits;
+    int splits, steps;  // splits of a tile's keys, steps of each
 };
-Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
+Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, int window, int sinks) {
     Plan p;
     const int group = n_heads / c.n_kv_heads;
     const int longest = b.max_rows > 0 ? std::min(b.max_rows, b.n_rows) : ceil_div(b.n_rows, b.n_seqs);
     const bool chunk = (int64_t)longest * group > 48;
     p.rows = chunk ? CR : 16;
     p.tiles = (int64_t)b.n_rows * group / p.rows + b.n_seqs;
-    // the tiles that hold rows when the sequences are as expected, their workgroups, and steps of the longest
+    // workgroups of the tiles that hold rows when the sequences are as expected, keys of the longest
     const int64_t expected = (int64_t)b.n_rows * group / p.rows + std::min(b.n_seqs, b.n_rows);
     const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
-    const int64_t want = (chunk ? 2 : 4) * (int64_t)n_cus / wgs;
-    const int64_t most = ceil_div<int64_t>(std::max(b.max_kv, 1), chunk ? 8 * CK : 4 * RW * RS);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, (int64_t)MAX_SPLITS}));
+    int64_t keys = std::max(b.max_kv, 1);
+    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + sinks + std::min<int64_t>(longest, p.rows));
+    const int64_t steps = ceil_div<int64_t>(keys, chunk ? CK : RS), least = chunk ? 8 : 4 * RW;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((chunk ? 2 : 4) * (int64_t)n_cus / wgs, MAX_SPLITS));
+    p.steps = (int)std::max<int64_t>(ceil_div(steps, want), least);
+    p.splits = (int)std::max<int64_t>(1, ceil_div<int64_t>(steps, p.steps));
     return p;
 }
 size_t plan_bytes(const Plan &p, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
@@ -730,11 +762,12 @@ size_t plan_bytes(const Plan &p, const mw_kv_cache &c, const mw_kv_batch &b, int
 
 }  // namespace
 
-size_t kv_attend_workspace(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
+size_t kv_attend_workspace(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, int window, int sinks) {
     check_kv(c, b);
     MW_CHECK(n_heads > 0 && n_heads % c.n_kv_heads == 0, "kv attend: n_heads is a multiple of n_kv_heads");
     if (b.n_rows == 0 || b.n_seqs == 0) return 0;
-    return plan_bytes(plan(n_cus, c, b, n_heads), c, b, n_heads);
+    MW_CHECK(window >= 0 && sinks >= 0, "kv attend: window and sinks are not negative");
+    return plan_bytes(plan(n_cus, c, b, n_heads, window, sinks), c, b, n_heads);
 }
 
 void check_kv_attend(const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendArgs &a) {
@@ -752,11 +785,11 @@ void check_kv_attend(const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendA
 void launch_kv_attend(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendArgs &a, hipStream_t st) {
     check_kv_attend(c, b, a);
     if (b.n_rows == 0 || b.n_seqs == 0) return;
-    const Plan p = plan(n_cus, c, b, a.n_heads);
+    const Plan p = plan(n_cus, c, b, a.n_heads, a.window, a.sinks);
     const size_t need = plan_bytes(p, c, b, a.n_heads);
     MW_CHECK(a.ws_bytes >= need && (need == 0 || (a.ws && (uintptr_t)a.ws % 16 == 0)), "kv attend: workspace too small or not 16-byte aligned");
     AttendP A{make_view(c, b), a.n_heads, a.n_heads / c.n_kv_heads, (const bf16_t *)a.q, a.q_row, a.q_head, (bf16_t *)a.out, a.o_row, a.o_head,
-              a.scale * 1.4426950408889634f, a.window, a.sinks, p.splits, (int)p.tiles, (float *)a.ws,
+              a.scale * 1.4426950408889634f, a.window, a.sinks, p.splits, p.steps, (int)p.tiles, (float *)a.ws,
               (float *)a.ws + (size_t)p.splits * b.n_rows * a.n_heads * c.head_dim};
     const int64_t blocks = p.tiles * c.n_kv_heads * p.splits;
     MW_CHECK(blocks < (1LL << 24), "kv attend: too many tiles");

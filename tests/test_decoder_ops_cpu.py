@@ -62,7 +62,7 @@ def test_caches_that_are_refused(pkg, field, value, why):
     for call in (_write, _attend):
         assert call(pkg, c, b) == -100
         assert why in pkg.last_error()
-    assert pkg.lib().mw_kv_attend_workspace(0, C.byref(c), C.byref(b), 4) == 0
+    assert pkg.lib().mw_kv_attend_workspace(0, C.byref(c), C.byref(b), 4, 0, 0) == 0
 
 
 @pytest.mark.parametrize("field,value,why", [

@@ -753,7 +753,7 @@ def test_refusals_on_the_gpu(pkg):
         import ctypes as C
         big = Case(pkg, "bf16", 64, 2, 16, [1], [4000])
         b = big.batch._for(big.cache.device, 1)
-        need = big.cache.L.mw_kv_attend_workspace(0, C.byref(big.cache.c), C.byref(b), 2)
+        need = big.cache.L.mw_kv_attend_workspace(0, C.byref(big.cache.c), C.byref(b), 2, 0, 0)
         assert need > 0
         pkg._call("attend", big.cache.L.mw_kv_attend_device(0, None, C.byref(big.cache.c), C.byref(b), 2, q.data_ptr(), 128, 64, q.data_ptr(), 128, 64,
                                                             0.1, 0, 0, q.data_ptr(), need - 1))
