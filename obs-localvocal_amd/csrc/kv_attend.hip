@@ -172,12 +172,21 @@ __device__ __forceinline__ int page_of_key(const KvView &V, int seq, int64_t j, 
 // Tiles of 16 rows: four waves take every fourth step of 32 keys; no wave waits for another before the end.  The next step's
 // rows are on their way while one is computed, their pages were looked up a step before (a key per lane).
 // ------------------------------------------------------------------------------------------------------------------------
+#ifndef ROWS_WANT
+#define ROWS_WANT 4
+#endif
+#ifndef CHUNK_WANT
+#define CHUNK_WANT 2
+#endif
+#ifndef ROWS_LEAST
+#define ROWS_LEAST 4
+#endif
 constexpr int RS = 32;      // keys per step
 constexpr int RW = 4;       // waves
 constexpr int VPAD = 16;    // V rows in LDS: 16 elements of padding put 8 consecutive rows on different banks for the transposing reads
 
 template <int KIND, int DH>
-__global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
+__global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void attend_rows_kernel(AttendP A) {
     constexpr int NS = DH / 32;        // 32-dim slices of the score product
     constexpr int ND = DH / 16;        // 16-dim tiles of the output
     constexpr int VLD = DH + VPAD;
@@ -191,7 +200,7 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
     __shared__ float sc[RW][2 * RS], pw[RW][KIND == INT8 ? 1 : RS * 16];
     __shared__ float ml[RW][16][2];
     const KvView &V = A.V;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
     const int split = blockIdx.x % A.splits;
     const int hk = (blockIdx.x / A.splits) % V.n_kv_heads, tile = blockIdx.x / A.splits / V.n_kv_heads;
     int seq, first;
@@ -246,59 +255,65 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
         if constexpr (KIND != BF16) x.scale = sbase[pg * V.s_page + r * V.s_row];  // lanes 0 .. 31 the keys', the others the values'
         x.dead = (unsigned)__ballot(page < 0);
     };
-    // one step; MASKED: some row may not see some key of it
-    auto step = [&](auto masked, Step &x, int64_t key0) {
-        constexpr bool MASKED = decltype(masked)::value;
+    // V rows (and scales) of a step -> LDS, keys that no row sees as zeros; whether one that some rows may not see is not finite
+    auto put = [&](const Step &x, bool whole) {
+        bool bad = false;
         if constexpr (KIND != BF16) sc[wave][lane] = x.scale;
-        // V rows -> LDS (dead ones as zeros)
+        auto row = [&](int t, int c) { return (u32x4 *)&U.vt[wave][(16 * t + fr) * VLD + c / FL * 32 * FL + 8 * FL * g + 8 * (c % FL)]; };
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const bool gone = MASKED && (x.dead >> (16 * t + fr)) & 1;
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int c = 0; c < NS; ++c) {
-                u32x4 y = fragment<KIND>(x.v[t][c / FL], c % FL);
-                if constexpr (MASKED) {
+            for (int c = 0; c < NS; ++c) *row(t, c) = fragment<KIND>(x.v[t][c / FL], c % FL);
+        if (!whole) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) y[q] = gone ? 0 : y[q];
+            for (int t = 0; t < 2; ++t) {
+                if ((x.dead >> (16 * t + fr)) & 1) {
+#pragma unroll
+                    for (int c = 0; c < NS; ++c) *row(t, c) = u32x4{0, 0, 0, 0};
+                } else if (KIND != INT8) {
+#pragma unroll
+                    for (int c = 0; c < NS; ++c) bad |= has_nonfinite(fragment<KIND>(x.v[t][c / FL], c % FL));
                 }
-                *(u32x4 *)&U.vt[wave][(16 * t + fr) * VLD + c / FL * 32 * FL + 8 * FL * g + 8 * (c % FL)] = y;
             }
         }
         __builtin_amdgcn_wave_barrier();  // what other lanes of the wave read below is written above (LDS keeps a wave's order)
-        // scores (taken out of the result vectors at once: an element set under a branch there was compiled wrongly)
-        float s[2][4];
+        return KIND != INT8 && __ballot(bad) != 0;
+    };
+    // scores (taken out of the result vectors at once: an element set under a branch there was compiled wrongly)
+    auto scores = [&](const Step &x, float (&s)[2][4]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NS; ++c)
-                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fragment<KIND>(x.k[t][c / FL], c % FL)), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fragment<KIND>(x.k[t][c / FL], c % FL)),
+                                                            __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = a[r] * (KIND == BF16 ? A.c : sc[wave][16 * t + 4 * g + r] * A.c);
         }
-        // the 32 keys this lane's row sees, a bit each
-        unsigned vis = ~0u;
-        if constexpr (MASKED) {
-            vis = ~x.dead & low_bits(p - key0 + 1);
-            if (A.window > 0) vis &= ~low_bits(p - A.window - key0 + 1) | low_bits((int64_t)A.sinks - key0);
-            const unsigned mine = vis >> (4 * g);  // bit 16 t + r: the lane's key r of tile t
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] = mine & (1u << (16 * t + r)) ? s[t][r] : -INFINITY;
-        }
-        // running maximum and sum
+    };
+    // the 32 keys this lane's row sees, a bit each
+    auto visible = [&](unsigned dead, int64_t key0) {
+        unsigned vis = ~dead & low_bits(p - key0 + 1);
+        if (A.window > 0) vis &= ~low_bits(p - A.window - key0 + 1) | low_bits((int64_t)A.sinks - key0);
+        return vis;
+    };
+    // running maximum and sum; s becomes the values' weights
+    auto softmax = [&](float (&s)[2][4], unsigned vis) {
+        const unsigned mine = vis >> (4 * g);  // bit 16 t + r: the lane's key r of tile t
         float mx = m;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
+            for (int r = 0; r < 4; ++r) {
+                s[t][r] = mine & (1u << (16 * t + r)) ? s[t][r] : -INFINITY;
+                mx = fmaxf(mx, s[t][r]);
+            }
         mx = xor_max<32>(xor_max<16>(mx));
         const float ref = mx == -INFINITY ? 0.0f : mx;  // nothing seen so far: exp2(-inf - 0) = 0
         const float corr = __builtin_amdgcn_exp2f(m - ref);
         m = mx;
         float ps = 0.0f;
-        float pv[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -306,75 +321,89 @@ __global__ __launch_bounds__(64 * RW, 2) void attend_rows_kernel(AttendP A) {
                 const float e = __builtin_amdgcn_exp2f(s[t][r] - ref);
                 ps += e;
                 // (the scale of a value that is not seen may be anything)
-                if constexpr (KIND == BF16) pv[t][r] = e;
-                else pv[t][r] = !MASKED || (vis >> (4 * g)) & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
+                if constexpr (KIND == BF16) s[t][r] = e;
+                else s[t][r] = mine & (1u << (16 * t + r)) ? e * sc[wave][RS + 16 * t + 4 * g + r] : 0.0f;
             }
         l = l * corr + ps;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= corr;
-        bool per_key = false;
-        if constexpr (KIND != INT8 && MASKED) {  // a value that some rows see and others do not must not reach the others: 0 x inf = NaN
-            bool bad = false;
+    };
+    // one step; whole: every row sees every key of it.  x takes the next step's rows as soon as this one's are used.
+    int page = -1;
+    bool left = false;  // steps with values that are not finite and that some rows do not see: done at the end
+    auto step = [&](Step &x, bool whole, int64_t key0, int next) {
+        unsigned dead = x.dead;
+        float s[2][4];
+        if (put(x, whole)) {
+            left = true;
+            dead = ~0u;  // (as if no row saw it)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int c = 0; c < NS; ++c) bad |= !((x.dead >> (16 * t + fr)) & 1) && has_nonfinite(fragment<KIND>(x.v[t][c / FL], c % FL));
-            per_key = __ballot(bad) != 0;
-        }
-        if (!per_key) {
-            // the residue of the probabilities' rounding goes through a second product: these kernels wait for memory, not for the MFMAs
-            const u32x4 pb = {pack_bf16(pv[0][0], pv[0][1]), pack_bf16(pv[0][2], pv[0][3]), pack_bf16(pv[1][0], pv[1][1]), pack_bf16(pv[1][2], pv[1][3])};
-            const u32x4 pl = low_part(&pv[0][0], pb);
-            const bf16_t *vb = &U.vt[wave][(4 * g + (fr >> 2)) * VLD + (fr & 3) * 4];
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * d)));
-                const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * VLD + 16 * d)));
-                const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
-            }
-        } else {  // key by key, rows that see it only
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) pw[wave][(16 * t + 4 * g + r) * 16 + fr] = pv[t][r];
+                for (int c = 0; c < NS; ++c)
+                    *(u32x4 *)&U.vt[wave][(16 * t + fr) * VLD + c / FL * 32 * FL + 8 * FL * g + 8 * (c % FL)] = u32x4{0, 0, 0, 0};
             __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-            for (int k = 0; k < RS; ++k) {
-                const float pk = pw[wave][k * 16 + fr];
-                const bf16_t *vrow = &U.vt[wave][k * VLD + 4 * g];
-                const bool ok = (vis >> k) & 1;
+        }
+        scores(x, s);
+        load(x, min(next, i1 - 1), page);
+        page = page_of(next + RW);
+        softmax(s, whole ? ~0u : visible(dead, key0));
+        // the residue of the probabilities' rounding goes through a second product: these kernels wait for memory, not for the MFMAs
+        const u32x4 pb = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+        const u32x4 pl = low_part(&s[0][0], pb);
+        const bf16_t *vb = &U.vt[wave][(4 * g + (fr >> 2)) * VLD + (fr & 3) * 4];
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float y = fmaf(pk, __uint_as_float((unsigned)vrow[16 * d + e] << 16), o[d][e]);
-                        o[d][e] = ok ? y : o[d][e];
-                    }
-            }
+        for (int d = 0; d < ND; ++d) {
+            const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * d)));
+            const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vb + 16 * VLD + 16 * d)));
+            const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
         }
         __builtin_amdgcn_wave_barrier();  // the next step's rows come after this one's reads
     };
-    auto run = [&](Step &x, int i) {
-        const int64_t key0 = step_key<RS>(ks, i);
-        const bool whole = x.dead == 0 && key0 + RS - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + RS <= A.sinks);
-        if (whole) step(std::false_type{}, x, key0);
-        else step(std::true_type{}, x, key0);
-    };
     if (i0 < i1) {
-        Step x, y;
-        int page = page_of(i0);
-        load(x, i0, page);
+        Step x;
+        load(x, i0, page_of(i0));
         page = page_of(i0 + RW);
-        for (int i = i0; i < i1; i += 2 * RW) {
-            load(y, min(i + RW, i1 - 1), page);
-            page = page_of(i + 2 * RW);
-            run(x, i);
-            if (i + RW >= i1) break;
-            load(x, min(i + 2 * RW, i1 - 1), page);
-            page = page_of(i + 3 * RW);
-            run(y, i + RW);
+        auto whole = [&](int64_t key0) {
+            return x.dead == 0 && key0 + RS - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + RS <= A.sinks);
+        };
+        for (int i = i0; i < i1; i += RW) {
+            const int64_t key0 = step_key<RS>(ks, i);
+            step(x, whole(key0), key0, i + RW);
+        }
+        if (KIND != INT8 && left) {
+            // 0 x inf = NaN in a product over rows that do and rows that do not see a value: key by key, rows that see it only
+#pragma unroll 1
+            for (int i = i0; i < i1; i += RW) {
+                const int64_t key0 = step_key<RS>(ks, i);
+                load(x, i, page_of(i));
+                if (whole(key0) || !put(x, false)) continue;
+                const unsigned vis = visible(x.dead, key0);
+                float s[2][4];
+                scores(x, s);
+                softmax(s, vis);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) pw[wave][(16 * t + 4 * g + r) * 16 + fr] = s[t][r];
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+                for (int k = 0; k < RS; ++k) {
+                    const float pk = pw[wave][k * 16 + fr];
+                    const bf16_t *vrow = &U.vt[wave][k * VLD + 4 * g];
+                    const bool ok = (vis >> k) & 1;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float y = fmaf(pk, __uint_as_float((unsigned)vrow[16 * d + e] << 16), o[d][e]);
+                            o[d][e] = ok ? y : o[d][e];
+                        }
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
         }
     }
     l = xor_sum<32>(xor_sum<16>(l));
@@ -444,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
     __shared__ __attribute__((aligned(16))) float sc[2][2][CK];
     __shared__ int odd[2];  // a buffer whose values are not all finite
     const KvView &V = A.V;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 31, h = lane >> 5;
     // tiles with the most keys first: in a chunk the later ones
     const int hk = blockIdx.x % V.n_kv_heads, rest = blockIdx.x / V.n_kv_heads;
     const int split = rest % A.splits, tile = A.tiles - 1 - rest / A.splits;
@@ -750,8 +779,8 @@ Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, in
     const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
     int64_t keys = std::max(b.max_kv, 1);
     if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + sinks + std::min<int64_t>(longest, p.rows));
-    const int64_t steps = ceil_div<int64_t>(keys, chunk ? CK : RS), least = chunk ? 8 : 4 * RW;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((chunk ? 2 : 4) * (int64_t)n_cus / wgs, MAX_SPLITS));
+    const int64_t steps = ceil_div<int64_t>(keys, chunk ? CK : RS), least = chunk ? 8 : ROWS_LEAST * RW;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((chunk ? CHUNK_WANT : ROWS_WANT) * (int64_t)n_cus / wgs, MAX_SPLITS));
     p.steps = (int)std::max<int64_t>(ceil_div(steps, want), least);
     p.splits = (int)std::max<int64_t>(1, ceil_div<int64_t>(steps, p.steps));
     return p;
