@@ -463,7 +463,7 @@ constexpr int CR = 128, CK = 64;  // rows, keys per step
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
 template <int KIND, int DH>
-__global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
+__global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_chunk_kernel(AttendP A) {
     constexpr int KLD = DH + 8, VLD = DH + 16;  // row strides in LDS: fragment reads without bank conflicts
     constexpr int EB = KIND == BF16 ? 2 : 1;
     constexpr int LPR = DH / 8, RPP = 256 / LPR, NP = CK / RPP;  // lanes per row, rows per pass, passes
@@ -558,11 +558,11 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
         store(0, !all_see(key0), dead);
     }
     __syncthreads();
-    // one step; MASKED: some row may not see some key of it
-    auto step = [&](auto masked, int cur, int64_t key0) {
+    // s: weights of the values of a step, with the running maximum and sum.  MASKED: some row may not see some key of it, vis gets
+    // the keys this lane's row sees; hide: none does
+    auto weights = [&](auto masked, int cur, int64_t key0, bool hide, float (&s)[2][16], unsigned (&vis)[2]) {
         constexpr bool MASKED = decltype(masked)::value;
-        const bf16_t *kb = kt[cur], *vb = vt[cur];
-        float s[2][16];
+        const bf16_t *kb = kt[cur];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 a;
@@ -586,11 +586,10 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
                     for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
                 }
         }
-        unsigned vis[2] = {~0u, ~0u};
         if constexpr (MASKED) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                unsigned v = ~(unsigned)(dead >> (32 * t)) & low_bits(p - key0 + 1 - 32 * t);
+                unsigned v = hide ? 0u : ~(unsigned)(dead >> (32 * t)) & low_bits(p - key0 + 1 - 32 * t);
                 if (A.window > 0) v &= ~low_bits(p - A.window - key0 + 1 - 32 * t) | low_bits((int64_t)A.sinks - key0 - 32 * t);
                 vis[t] = v;
                 const unsigned mine = v >> (4 * h);
@@ -643,46 +642,28 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
                     for (int r = 0; r < 16; ++r) s[t][r] = (vis[t] >> (4 * h)) & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : 0.0f;
             }
         }
-        if (KIND == INT8 || !MASKED || odd[cur] == 0) {
-            const int gi = lane >> 4, ii = lane & 15;
-            const bf16_t *va = vb + (4 * h + (ii >> 2)) * VLD + 16 * (gi & 1) + (ii & 3) * 4;
+    };
+    auto products = [&](int cur, const float (&s)[2][16]) {
+        const int gi = lane >> 4, ii = lane & 15;
+        const bf16_t *va = vt[cur] + (4 * h + (ii >> 2)) * VLD + 16 * (gi & 1) + (ii & 3) * 4;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float *e = &s[c >> 1][8 * (c & 1)];
-                const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
-                u32x4 pl = {0, 0, 0, 0};
-                if constexpr (KIND == INT8) pl = low_part(e, pb);
+        for (int c = 0; c < 4; ++c) {
+            const float *e = &s[c >> 1][8 * (c & 1)];
+            const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
+            u32x4 pl = {0, 0, 0, 0};
+            if constexpr (KIND == INT8) pl = low_part(e, pb);  // (a code's scale leaves the largest weight no power of two: its rounding would show)
 #pragma unroll
-                for (int d = 0; d < DH / 32; ++d) {
-                    const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + 16 * c * VLD + 32 * d)));
-                    const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + (16 * c + 8) * VLD + 32 * d)));
-                    const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
-                    if constexpr (KIND == INT8)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
-                }
-            }
-        } else {
-            // values that are not finite and that some rows do not see (0 x inf = NaN): key by key, rows that see it only
-#pragma unroll 1
-            for (int k = 0; k < CK; ++k) {
-                const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the 32 of its half
-                float mine = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
-                const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
-                const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
-                const bf16_t *vrow = vb + k * VLD + 4 * h;
-#pragma unroll
-                for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        const float x = fmaf(pk, __uint_as_float((unsigned)vrow[32 * d + 8 * (q >> 2) + (q & 3)] << 16), o[d][q]);
-                        o[d][q] = ok ? x : o[d][q];
-                    }
+            for (int d = 0; d < DH / 32; ++d) {
+                const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + 16 * c * VLD + 32 * d)));
+                const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + (16 * c + 8) * VLD + 32 * d)));
+                const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+                if constexpr (KIND == INT8)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
             }
         }
     };
+    bool left = false;  // steps with values that are not finite and that some rows do not see: done at the end
     int i = i0, cur = 0;
     // the next step's loads, this one, the next one's rows into the other buffer (last read before the previous barrier)
     auto advance = [&](auto masked) {
@@ -691,7 +672,14 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
         dead_n = __ballot(page_n < 0);
         load(step_key<CK>(ks, more ? i + 1 : i), page_n);  // (behind the last step: loaded, not used)
         page_n = page_of(i + 2);
-        step(masked, cur, key0);
+        {
+            float s[2][16];
+            unsigned vis[2];
+            const bool hide = KIND != INT8 && decltype(masked)::value && odd[cur] != 0;
+            left |= hide;
+            weights(masked, cur, key0, hide, s, vis);
+            if (!hide) products(cur, s);
+        }
         const bool check = more && !all_see(step_key<CK>(ks, i + 1));
         if (KIND != INT8) {
             if (check) {
@@ -710,6 +698,44 @@ __global__ __launch_bounds__(256, 2) void attend_chunk_kernel(AttendP A) {
     while (i < i1) {
         while (i < i1 && dead == 0 && all_see(step_key<CK>(ks, i))) advance(std::false_type{});
         if (i < i1) advance(std::true_type{});
+    }
+    if (KIND != INT8 && left) {
+        // 0 x inf = NaN in a product over rows that do and rows that do not see a value: key by key, rows that see it only
+#pragma unroll 1
+        for (i = i0; i < i1; ++i) {
+            const int64_t key0 = step_key<CK>(ks, i);
+            const int pg = page_of(i);
+            dead = __ballot(pg < 0);
+            if (dead == 0 && all_see(key0)) continue;
+            if (tid == 0) odd[0] = 0;
+            load(key0, pg);
+            __syncthreads();
+            store(0, true, dead);
+            __syncthreads();
+            if (odd[0] != 0) {
+                float s[2][16];
+                unsigned vis[2];
+                weights(std::true_type{}, 0, key0, false, s, vis);
+#pragma unroll 1
+                for (int k = 0; k < CK; ++k) {
+                    const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the 32 of its half
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
+                    const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
+                    const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
+                    const bf16_t *vrow = vt[0] + k * VLD + 4 * h;
+#pragma unroll
+                    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            const float x = fmaf(pk, __uint_as_float((unsigned)vrow[32 * d + 8 * (q >> 2) + (q & 3)] << 16), o[d][q]);
+                            o[d][q] = ok ? x : o[d][q];
+                        }
+                }
+            }
+            __syncthreads();
+        }
     }
     l += __shfl_xor(l, 32);
     if (wave * 32 + fr >= n_tile) return;
