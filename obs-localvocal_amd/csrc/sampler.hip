@@ -28,7 +28,6 @@ constexpr int SW = ST / 64;       // waves
 constexpr int NB = 2048;          // bins
 constexpr int LIST = 1024;        // tokens of a list, one a thread (a place takes 10 bits beside an index)
 constexpr int FEW = 512;          // a cut of top-k up to here is looked for among the largest tokens
-constexpr int GUESS = 384;        // threads whose largest token the list of the likeliest is to hold when no top-k says how many
 constexpr double LN2 = 0.6931471805599453;
 
 struct Shared {
@@ -42,7 +41,7 @@ struct Shared {
     u64 lo, hi;                   // key range of a division
     u64 cut, cut_mass;            // last kept key, weight up to and including it
     u64 found_mass;               // weight before the bin found
-    u64 kept, total;
+    u64 kept, total, extra[SW];
     unsigned found_bin, found_before, found_count, n_list;
 };
 
@@ -117,8 +116,8 @@ __device__ __forceinline__ double block_sum_f(Shared &S, float v) {
     return t;
 }
 // A value that at least `want` of the threads' largest values reach, and not many more: bisection between the row's maximum and
-// 2^-32 of its weight, by one wave (16 values a lane, counted by ballots: no barrier inside).  -FLT_MAX when that many do not
-// exist there.
+// 2^-32 of its weight, by one wave (no barrier inside).  Up to a quarter of 256 it looks at the largest of every four threads.
+// -FLT_MAX when that many do not exist there.
 __device__ __forceinline__ float bound_of(Shared &S, float mine, const Row &R, int want) {
     S.most[threadIdx.x] = mine;
     __syncthreads();
@@ -126,10 +125,19 @@ __device__ __forceinline__ float bound_of(Shared &S, float mine, const Row &R, i
         float v[SW];
 #pragma unroll
         for (int i = 0; i < SW; ++i) v[i] = S.most[i * 64 + threadIdx.x];
+        const bool few = want <= 64;
+        if (few) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = fmaxf(fmaxf(v[i], v[i + 4]), fmaxf(v[i + 8], v[i + 12]));
+        }
         auto reach = [&](float x) {
             int n = 0;
 #pragma unroll
-            for (int i = 0; i < SW; ++i) n += __popcll(__ballot(v[i] >= x));
+            for (int i = 0; i < 4; ++i) n += __popcll(__ballot(v[i] >= x));
+            if (!few) {
+#pragma unroll
+                for (int i = 4; i < SW; ++i) n += __popcll(__ballot(v[i] >= x));
+            }
             return n;
         };
         float hi = R.max, lo = fmaxf(R.max - 32.0f / R.c, -3.4028235e38f);
@@ -281,6 +289,7 @@ template <bool BF> struct Source {
         K = ((nc + SW - 1) / SW + 63) / 64;
         c0 = (threadIdx.x >> 6) * K * 64 + (threadIdx.x & 63);
     }
+    __device__ __forceinline__ int owner(int i) const { return (i + mis) / VEC / (64 * K); }  // the wave that has token i
     __device__ __forceinline__ int first(int k) const { return (c0 + 64 * k) * VEC - mis; }
     // the values from index i0 on; what lies outside the row is -inf and never read
     __device__ __forceinline__ void load(int i0, float (&v)[VEC]) const {
@@ -327,8 +336,10 @@ template <bool BF> struct Source {
 };
 
 // The last kept token when the order is cut at `want` (a count or a weight): S.cut (its key) and S.cut_mass (weight up to and with it).
+// On the way mine gets the thread's share of what is kept ahead of the list (tokens of at least `least`), S.extra what is kept of the
+// list for the wave that owns the token.
 template <bool BY_COUNT, typename SRC>
-__device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R, double want) {
+__device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R, double want, float least, double &mine) {
     find_bin<BY_COUNT>(S, S.cnt, S.mass, 0, 0, want);
     const int bin = (int)S.found_bin;
     unsigned before = S.found_before;
@@ -342,18 +353,30 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
     auto gather = [&]() -> unsigned {
         __syncthreads();
         if (threadIdx.x == 0) S.n_list = 0;
+        if (threadIdx.x < SW) S.extra[threadIdx.x] = 0;
         __syncthreads();
-        src.each([&](float x, int i) {
-            if (in_bin(x)) {
-                const u64 r = rank_key(x, i);
-                if (r >= lo && r <= hi) {
-                    const unsigned at = atomicAdd(&S.n_list, 1u);
-                    if (at < LIST) {
-                        S.list_r[at] = r;
-                        S.list_w[at] = R.weight32(x);
+        mine = 0.0;
+        src.pieces([&](const float (&v)[SRC::VEC], int i0, int) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < SRC::VEC; ++e) {
+                const float q = R.power(v[e]);
+                if (q > end) {
+                    const float w = __builtin_amdgcn_exp2f(q);
+                    bool ahead = q > top;
+                    if (!ahead) {
+                        const u64 r = rank_key(v[e], i0 + e);
+                        ahead = r < lo;
+                        if (!ahead && r <= hi) {
+                            const unsigned at = atomicAdd(&S.n_list, 1u);
+                            if (at < LIST) S.list_r[at] = r;
+                        }
                     }
+                    sum += ahead && w >= least ? w : 0.0f;
                 }
             }
+            mine += (double)sum;
+            return true;
         });
         __syncthreads();
         return S.n_list;
@@ -413,7 +436,8 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
     // the list in order; the cut is where the running count or weight passes `want`
     const int n = (int)min(S.n_list, (unsigned)LIST), tid = threadIdx.x;
     const u64 key = block_sort(S, tid < n ? placed_key(S.list_r[tid], tid) : ~0ull, n);
-    const u64 w = tid < n ? S.list_w[key & (LIST - 1)] : 0;
+    const float x = key_value(key);
+    const u64 w = tid < n ? R.weight32(x) : 0;
     const u64 mass = before_mass + block_scan(S, w, n);
     if (tid < n) {
         const bool ahead = BY_COUNT ? (double)(before + tid) < want : (double)(mass - w) < want;
@@ -422,6 +446,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
             S.cut = (key >> 32) << 32 | ((unsigned)key >> 10);
             S.cut_mass = mass;
         }
+        if (ahead && R.share(x) >= least) atomicAdd(&S.extra[src.owner((int)((unsigned)key >> 10))], R.weight(x));
     }
     __syncthreads();
 }
@@ -454,21 +479,58 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     R.c_d = fmin(fmax(1.4426950408889634 / (greedy ? 1.0 : (double)temp), 1e-30), 1e37);
     R.c = (float)R.c_d;
 
-    // ---- 2: total weight; the likeliest tokens into a list ----
+    // ---- 2: total weight; the likeliest tokens into a list, or a histogram ----
     const bool use_k = !greedy && k > 0 && k < A.n_vocab, use_p = !greedy && top_p < 1.0f, use_m = !greedy && min_p > 0.0f;
+    const float least = use_m ? fminf(min_p, 1.0f) : 0.0f;  // (the likeliest token's share is 1)
     float bound = INFINITY;
     if (greedy) bound = mx;
-    else if (use_k && k <= FEW) bound = bound_of(S, my_max, R, k);
-    else if (use_p || use_m) bound = bound_of(S, my_max, R, GUESS);
+    else if (use_k) bound = k <= FEW ? bound_of(S, my_max, R, k) : INFINITY;
+    else if (use_m && !use_p) bound = mx + (__builtin_amdgcn_logf(least) - 1e-5f) / R.c;  // (log2; a little more than what is kept)
     bound = fmaxf(bound, -3.4028235e38f);  // (-inf is never listed)
+    const bool lists = bound < INFINITY;
     float zf = 0.0f;
-    src.each([&](float x, int i) {
-        zf += R.share(x);
-        if (x >= bound) {
-            const unsigned at = atomicAdd(&S.n_list, 1u);
-            if (at < LIST) S.list_r[at] = rank_key(x, i);
+    // histogram over 64 d: counts if top-k asks for them, weights if top-p does.  The last bin takes all that is far away: in
+    // registers first, or its one address would be waited for by every lane.
+    auto histogram = [&]() {
+        for (int b = tid; b < NB; b += ST) {
+            S.cnt[b] = 0;
+            S.mass[b] = 0;
         }
-    });
+        __syncthreads();
+        unsigned far = 0;
+        u64 far_mass = 0;
+        src.each([&](float x, int) {
+            const float q = R.power(x), w = __builtin_amdgcn_exp2f(q);
+            zf += w;
+            const unsigned w32 = (unsigned)fmaf(w, 2147483648.0f, 0.5f);
+            if (q > -(float)(NB - 1) / 64.0f) {
+                const int b = (int)(-64.0f * q);
+                if (use_k) atomicAdd(&S.cnt[b], 1u);
+                if (use_p) atomicAdd(&S.mass[b], (u64)w32);
+            } else if (x > -INFINITY) {
+                ++far;
+                far_mass += w32;
+            }
+        });
+        if (far) {
+            atomicAdd(&S.cnt[NB - 1], far);
+            atomicAdd(&S.mass[NB - 1], far_mass);
+        }
+        __syncthreads();
+    };
+    if (lists) {
+        src.each([&](float x, int i) {
+            zf += R.share(x);
+            if (x >= bound) {
+                const unsigned at = atomicAdd(&S.n_list, 1u);
+                if (at < LIST) S.list_r[at] = rank_key(x, i);
+            }
+        });
+    } else if (use_k || use_p) {
+        histogram();
+    } else {
+        src.each([&](float x, int) { zf += R.share(x); });
+    }
     const double z = block_sum_f(S, zf);
     // a NaN anywhere is one in the sum; with a maximum of +inf or -inf nothing can be drawn
     if (z != z || !(mx < INFINITY) || mx == -INFINITY || temp != temp || top_p != top_p || min_p != min_p || u != u) {
@@ -494,23 +556,9 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     }
     const u64 me = tid < n ? S.list_r[tid] : ~0ull;
     const float listed_x = key_value(me);
-    const u64 w = tid < n ? R.weight(listed_x) : 0;
-    S.list_w[tid] = w;
-    // Does the list hold everything that is kept?
-    bool listed = bound < INFINITY && S.n_list <= LIST && !greedy;
-    if (listed && bound > -3.4028235e38f) {
-        if (use_k && k <= FEW) {
-            listed = n >= k;
-        } else if (use_k) {
-            listed = false;
-        } else if (use_p) {
-            u64 zb = w, t = 0;
-            block_sum64(S, zb, t);
-            listed = (double)zb >= (1.0 + 1e-6) * (double)top_p * z * 0x1p40;
-        } else {
-            listed = R.share(bound) < 0.999999f * min_p;
-        }
-    }
+    S.list_w[tid] = tid < n ? R.weight(listed_x) : 0;
+    // (a list that ran over: equal or very near tokens in numbers; the histogram then divides them)
+    const bool listed = lists && !greedy && S.n_list <= LIST;
     if (listed) {
         // in the order of the tokens: what is kept is a stretch from the first on
         u64 key = block_sort(S, tid < n ? placed_key(me, tid) : ~0ull, n);
@@ -526,7 +574,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
             }
             keep &= tid == 0 || (double)(upto - wt) < (double)top_p * kept;
         }
-        if (use_m) keep &= x == mx || R.share(x) >= min_p;
+        keep &= R.share(x) >= least;
         const int nk = block_count(S, keep);
         // in the order of the index: the draw
         key = block_sort(S, tid < nk ? (u64)(unsigned)key : ~0ull, nk);
@@ -546,53 +594,32 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     // ---- 3: cuts ----
     u64 cut = ~0ull;
     if (greedy) cut = (u64)(~ordered(mx)) << 32 | 0x7fffffffu;  // more equal largest logits than the list holds: the first of them is drawn
+    double mine = 0.0;
     if (use_k || use_p) {
-        for (int b = tid; b < NB; b += ST) {
-            S.cnt[b] = 0;
-            S.mass[b] = 0;
-        }
-        __syncthreads();
-        // (the last bin takes all that is far away: in registers first, or its one address would be waited for by every lane)
-        unsigned far = 0;
-        u64 far_mass = 0;
-        src.each([&](float x, int) {
-            const float q = -64.0f * R.power(x);
-            if (q < (float)(NB - 1)) {
-                if (use_k) atomicAdd(&S.cnt[(int)q], 1u);
-                if (use_p) atomicAdd(&S.mass[(int)q], (u64)R.weight32(x));
-            } else if (x > -INFINITY) {
-                ++far;
-                far_mass += R.weight32(x);
-            }
-        });
-        if (far) {
-            atomicAdd(&S.cnt[NB - 1], far);
-            atomicAdd(&S.mass[NB - 1], far_mass);
-        }
-        __syncthreads();
+        if (lists) histogram();
         double kept = z * 0x1p31;
         if (use_k) {
             // fewer tokens than k may be left by the suppressed ones: nothing to cut then
             u64 live = S.cnt[2 * tid] + S.cnt[2 * tid + 1], t = 0;
             block_sum64(S, live, t);
             if ((u64)k < live) {
-                resolve<true>(S, src, R, (double)k);
+                resolve<true>(S, src, R, (double)k, least, mine);
                 cut = S.cut;
                 kept = (double)S.cut_mass;
             }
         }
         if (use_p) {
             __syncthreads();
-            resolve<false>(S, src, R, fmax((double)top_p * kept, 0.5));
+            resolve<false>(S, src, R, fmax((double)top_p * kept, 0.5), least, mine);
             cut = S.cut;
         }
     }
+    const bool have_sums = (use_k || use_p) && cut != ~0ull;
 
     // ---- 4: draw ----
     const float cut_x = cut == ~0ull ? -INFINITY : key_value(cut);
     const int cut_i = cut == ~0ull ? 0x7fffffff : (int)(unsigned)cut;
     constexpr int VEC = Source<BF>::VEC;
-    const float least = use_m ? fminf(min_p, 1.0f) : 0.0f;  // (the likeliest token's share is 1)
     auto weight_kept = [&](float x, int i) -> float {
         const float w = R.share(x);
         const bool keep = x > cut_x || (x == cut_x && i <= cut_i);
@@ -604,17 +631,16 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
         for (int e = 0; e < VEC; ++e) s += weight_kept(v[e], i0 + e);
         return s;
     };
-    // (nothing dropped: the sums of the waves are those of step 2)
+    // (nothing dropped: the sums of the waves are those of step 2; after a cut they were formed on the way)
     const bool all_kept = !use_k && !use_p && !use_m && !greedy;
-    double mine = 0.0;
-    if (!all_kept) src.pieces([&](const float (&v)[VEC], int i0, int) {
+    if (!all_kept && !have_sums) src.pieces([&](const float (&v)[VEC], int i0, int) {
         mine += (double)piece_kept(v, i0);
         return true;
     });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
     __syncthreads();
-    if (lane == 0) S.wave_d[wave] = all_kept ? (double)S.wave_f[wave] : mine;
+    if (lane == 0) S.wave_d[wave] = all_kept ? (double)S.wave_f[wave] : have_sums ? mine + (double)S.extra[wave] * 0x1p-40 : mine;
     __syncthreads();
     double total = 0.0;
 #pragma unroll
