@@ -291,6 +291,7 @@ template <bool BF> struct Source {
     }
     __device__ __forceinline__ int owner(int i) const { return (i + mis) / VEC / (64 * K); }  // the wave that has token i
     __device__ __forceinline__ int first(int k) const { return (c0 + 64 * k) * VEC - mis; }
+    __device__ __forceinline__ int first(int w, int k) const { return ((w * K + k) * 64 + (int)(threadIdx.x & 63)) * VEC - mis; }  // of wave w
     // the values from index i0 on; what lies outside the row is -inf and never read
     __device__ __forceinline__ void load(int i0, float (&v)[VEC]) const {
         if (i0 >= 0 && i0 + VEC <= n) {
@@ -336,9 +337,9 @@ template <bool BF> struct Source {
 };
 
 // The last kept token when the order is cut at `want` (a count or a weight): S.cut (its key) and S.cut_mass (weight up to and with it).
-// On the way mine gets the thread's share of what is kept ahead of the list (tokens of at least `least`), S.extra what is kept of the
+// On the way (SUMS) mine gets the thread's share of what is kept ahead of the list (tokens of at least `least`), S.extra what is kept of the
 // list for the wave that owns the token.
-template <bool BY_COUNT, typename SRC>
+template <bool BY_COUNT, bool SUMS, typename SRC>
 __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R, double want, float least, double &mine) {
     find_bin<BY_COUNT>(S, S.cnt, S.mass, 0, 0, want);
     const int bin = (int)S.found_bin;
@@ -360,22 +361,19 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < SRC::VEC; ++e) {
-                const float q = R.power(v[e]);
-                if (q > end) {
-                    const float w = __builtin_amdgcn_exp2f(q);
-                    bool ahead = q > top;
-                    if (!ahead) {
-                        const u64 r = rank_key(v[e], i0 + e);
-                        ahead = r < lo;
-                        if (!ahead && r <= hi) {
-                            const unsigned at = atomicAdd(&S.n_list, 1u);
-                            if (at < LIST) S.list_r[at] = r;
-                        }
+                const float q = R.power(v[e]), w = SUMS ? __builtin_amdgcn_exp2f(q) : 0.0f;
+                if (SUMS) sum += q > top && w >= least ? w : 0.0f;
+                if (q > end && q <= top) {  // (few)
+                    const u64 r = rank_key(v[e], i0 + e);
+                    if (r < lo) {
+                        if (SUMS) sum += w >= least ? w : 0.0f;
+                    } else if (r <= hi) {
+                        const unsigned at = atomicAdd(&S.n_list, 1u);
+                        if (at < LIST) S.list_r[at] = r;
                     }
-                    sum += ahead && w >= least ? w : 0.0f;
                 }
             }
-            mine += (double)sum;
+            if (SUMS) mine += (double)sum;
             return true;
         });
         __syncthreads();
@@ -446,7 +444,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
             S.cut = (key >> 32) << 32 | ((unsigned)key >> 10);
             S.cut_mass = mass;
         }
-        if (ahead && R.share(x) >= least) atomicAdd(&S.extra[src.owner((int)((unsigned)key >> 10))], R.weight(x));
+        if (SUMS && ahead && R.share(x) >= least) atomicAdd(&S.extra[src.owner((int)((unsigned)key >> 10))], R.weight(x));
     }
     __syncthreads();
 }
@@ -603,14 +601,15 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
             u64 live = S.cnt[2 * tid] + S.cnt[2 * tid + 1], t = 0;
             block_sum64(S, live, t);
             if ((u64)k < live) {
-                resolve<true>(S, src, R, (double)k, least, mine);
+                if (use_p) resolve<true, false>(S, src, R, (double)k, least, mine);
+                else resolve<true, true>(S, src, R, (double)k, least, mine);
                 cut = S.cut;
                 kept = (double)S.cut_mass;
             }
         }
         if (use_p) {
             __syncthreads();
-            resolve<false>(S, src, R, fmax((double)top_p * kept, 0.5), least, mine);
+            resolve<false, true>(S, src, R, fmax((double)top_p * kept, 0.5), least, mine);
             cut = S.cut;
         }
     }
@@ -661,21 +660,32 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
         }
         run += s;
     }
+    if (owner < 0) return;  // (not reached: the likeliest token has weight)
+    // the tiles of its piece, shared by all waves
+    for (int kk = wave; kk < src.K; kk += SW) {
+        float v[VEC];
+        const int i0 = src.first(owner, kk);
+        src.load(i0, v);
+        const float s = wave_sum_desc(piece_kept(v, i0));
+        if (lane == 0) S.most[kk] = s;
+    }
+    __syncthreads();
     if (wave != owner) return;  // one wave goes on
     run = below;
     int tile = 0;
     double tile_run = below;
-    src.pieces([&](const float (&v)[VEC], int i0, int kk) {
-        const double s = (double)wave_sum_desc(piece_kept(v, i0));
+    done = false;
+    for (int kk = 0; kk < src.K && !done; ++kk) {
+        const double s = (double)S.most[kk];
         if (s > 0.0) {
             tile = kk;
             tile_run = run;
         }
         run += s;
-        return !(s > 0.0 && run >= target);
-    });
+        done = s > 0.0 && run >= target;
+    }
     float v[VEC];
-    const int i0 = src.first(tile);
+    const int i0 = src.first(owner, tile);
     src.load(i0, v);
     const double s = (double)piece_kept(v, i0);
     double incl = s;
