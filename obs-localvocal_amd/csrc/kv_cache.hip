@@ -58,10 +58,14 @@ template <int KIND> __host__ __device__ constexpr int elem_bytes() { return KIND
 
 __device__ __forceinline__ unsigned pack_bf16(float a, float b) { return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2)); }
 
+// A lane's 8 elements of a row: adjacent ones where rows come and go as bf16; 4 and 4, half a row apart, where they do as fp32, so
+// that every load and store of 16 bytes a lane covers whole lines (two of them 16 bytes apart wrote every line twice by halves).
+template <bool F32, int DH> __device__ __forceinline__ int first_of(int sub) { return sub * (F32 ? 4 : 8); }
+
 // 8 elements of a row of bf16 or fp32
-template <bool F32> __device__ __forceinline__ void load8(const void *p, int64_t at, float (&x)[8]) {
+template <bool F32, int DH> __device__ __forceinline__ void load8(const void *p, int64_t at, float (&x)[8]) {
     if constexpr (F32) {
-        const f32x4 a = *(const f32x4 *)((const float *)p + at), b = *(const f32x4 *)((const float *)p + at + 4);
+        const f32x4 a = *(const f32x4 *)((const float *)p + at), b = *(const f32x4 *)((const float *)p + at + DH / 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[i] = a[i];
@@ -76,10 +80,10 @@ template <bool F32> __device__ __forceinline__ void load8(const void *p, int64_t
         }
     }
 }
-template <bool F32> __device__ __forceinline__ void store8(void *p, int64_t at, const float (&x)[8]) {
+template <bool F32, int DH> __device__ __forceinline__ void store8(void *p, int64_t at, const float (&x)[8]) {
     if constexpr (F32) {
         *(f32x4 *)((float *)p + at) = f32x4{x[0], x[1], x[2], x[3]};
-        *(f32x4 *)((float *)p + at + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        *(f32x4 *)((float *)p + at + DH / 2) = f32x4{x[4], x[5], x[6], x[7]};
     } else {
         *(u32x4 *)((bf16_t *)p + at) = u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
     }
@@ -110,9 +114,16 @@ __device__ __forceinline__ int int8_code(float x, float scale, float inv) {
     return (int)q;
 }
 
-template <int KIND, int DH> __device__ __forceinline__ void write_row(char *dst, float *scale_at, const float (&x)[8], int sub) {
+template <int KIND, int DH, bool F32> __device__ __forceinline__ void write_row(char *dst, float *scale_at, const float (&x)[8], int sub) {
+    dst += first_of<F32, DH>(sub) * elem_bytes<KIND>();
     if constexpr (KIND == BF16) {
-        *(u32x4 *)(dst + sub * 16) = u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+        const u32x4 c = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+        if constexpr (F32) {
+            *(u32x2 *)dst = u32x2{c.x, c.y};
+            *(u32x2 *)(dst + DH) = u32x2{c.z, c.w};
+        } else {
+            *(u32x4 *)dst = c;
+        }
     } else {
         const unsigned ub = row_amax_bits<DH>(x);
         const bool bad = ub >= 0x7f800000u;
@@ -142,20 +153,34 @@ template <int KIND, int DH> __device__ __forceinline__ void write_row(char *dst,
             }
         }
         if (bad) scale = __uint_as_float(0x7fc00000u);
-        *(u32x2 *)(dst + sub * 8) = code;
+        if constexpr (F32) {
+            *(unsigned *)dst = code.x;
+            *(unsigned *)(dst + DH / 2) = code.y;
+        } else {
+            *(u32x2 *)dst = code;
+        }
         if (sub == 0) *scale_at = scale;
     }
 }
-template <int KIND> __device__ __forceinline__ void read_row(const char *src, const float *scale_at, float (&x)[8], int sub) {
+template <int KIND, int DH, bool F32> __device__ __forceinline__ void read_row(const char *src, const float *scale_at, float (&x)[8], int sub) {
+    src += first_of<F32, DH>(sub) * elem_bytes<KIND>();
     if constexpr (KIND == BF16) {
-        const u32x4 a = *(const u32x4 *)(src + sub * 16);
+        u32x4 a;
+        if constexpr (F32) {
+            const u32x2 lo = *(const u32x2 *)src, hi = *(const u32x2 *)(src + DH);
+            a = u32x4{lo.x, lo.y, hi.x, hi.y};
+        } else {
+            a = *(const u32x4 *)src;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[2 * i] = __uint_as_float(a[i] << 16);
             x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
         }
     } else {
-        const u32x2 c = *(const u32x2 *)(src + sub * 8);
+        u32x2 c;
+        if constexpr (F32) c = u32x2{*(const unsigned *)src, *(const unsigned *)(src + DH / 2)};
+        else c = *(const u32x2 *)src;
         const float s = *scale_at;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -188,24 +213,24 @@ __global__ __launch_bounds__(KT) void kv_rows_kernel(KvView V, const void *__res
     if (b < 0) return;
     const int64_t p = (int64_t)V.kv_len[b] - ((int64_t)V.cu[b + 1] - t);
     const int page = p >= 0 ? kv_page(V, b, p) : -1;
-    const int64_t at = t * row_stride + h * head_stride + sub * 8;
+    const int64_t at = t * row_stride + h * head_stride + first_of<F32, DH>(sub);
     const int64_t off = page * V.page_stride + h * V.head_stride + (p & V.mask) * V.row_stride;
     const int64_t soff = page * V.s_page + h * V.s_head + (p & V.mask) * V.s_row;
     if constexpr (WRITE) {
         if (page < 0) return;
         float x[8], y[8];
-        load8<F32>(kr, at, x);
-        load8<F32>(vr, at, y);
-        write_row<KIND, DH>(V.k + off * elem_bytes<KIND>(), V.ks + soff, x, sub);
-        write_row<KIND, DH>(V.v + off * elem_bytes<KIND>(), V.vs + soff, y, sub);
+        load8<F32, DH>(kr, at, x);
+        load8<F32, DH>(vr, at, y);
+        write_row<KIND, DH, F32>(V.k + off * elem_bytes<KIND>(), V.ks + soff, x, sub);
+        write_row<KIND, DH, F32>(V.v + off * elem_bytes<KIND>(), V.vs + soff, y, sub);
     } else {
         float x[8] = {}, y[8] = {};
         if (page >= 0) {
-            read_row<KIND>(V.k + off * elem_bytes<KIND>(), V.ks + soff, x, sub);
-            read_row<KIND>(V.v + off * elem_bytes<KIND>(), V.vs + soff, y, sub);
+            read_row<KIND, DH, F32>(V.k + off * elem_bytes<KIND>(), V.ks + soff, x, sub);
+            read_row<KIND, DH, F32>(V.v + off * elem_bytes<KIND>(), V.vs + soff, y, sub);
         }
-        store8<F32>(kw, at, x);
-        store8<F32>(vw, at, y);
+        store8<F32, DH>(kw, at, x);
+        store8<F32, DH>(vw, at, y);
     }
 }
 
