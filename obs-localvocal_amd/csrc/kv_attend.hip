@@ -101,6 +101,10 @@ __device__ __forceinline__ bool has_nonfinite(u32x4 x) {  // of 8 bf16
     return bad != 0;
 }
 
+// A value that is the same in all lanes, for the compiler to know: what follows from it (a step's keys, the loops' ends) then stays
+// in scalar registers.
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // The tile of `tile_rows` rows a workgroup has: its sequence and the first row inside it.  Sequences are cut into tiles one
 // after the other; every wave looks through 64 sequences at a time.
 __device__ __forceinline__ bool find_tile(const KvView &V, int group, int tile_rows, int tile, int &seq, int &first_row) {
@@ -119,12 +123,12 @@ __device__ __forceinline__ bool find_tile(const KvView &V, int group, int tile_r
             const int u = __shfl_up(incl, o);
             if (lane >= o) incl += u;
         }
-        const int all = __shfl(incl, 63);
+        const int all = scalar(__shfl(incl, 63));
         if (tile - base < all) {
             const unsigned long long m = __ballot(base + incl > tile);
             const int l = __ffsll((unsigned long long)m) - 1;
-            seq = __builtin_amdgcn_readfirstlane(s0 + l);
-            first_row = __builtin_amdgcn_readfirstlane((tile - base - __shfl(incl - n, l)) * tile_rows);
+            seq = scalar(s0 + l);
+            first_row = scalar((tile - base - __shfl(incl - n, l)) * tile_rows);
             return true;
         }
         base += all;
@@ -160,12 +164,12 @@ __device__ __forceinline__ KeyRange split_steps(int n, int split, const AttendP 
     return {(int)min(b, (int64_t)n), split == A.splits - 1 ? n : (int)min(e, (int64_t)n)};
 }
 
-// The page of key j, or -1 (j is anything below 2^62; a table has at least one column where there are keys).  No branch: the
-// entry is loaded in any case, from a column that exists.
-__device__ __forceinline__ int page_of_key(const KvView &V, int seq, int64_t j, bool wanted) {
+// The table's entry for key j (anything below 2^62; a table has at least one column where there are keys).  No branch: it is loaded
+// in any case, from a column that exists, and looked at only when the key's rows are loaded, a step later: a check beside the load
+// waited for it, and with it for every row on its way.
+__device__ __forceinline__ int page_entry(const KvView &V, int seq, int64_t j) {
     const int64_t col = min(max(j, (int64_t)0) >> V.shift, (int64_t)V.table_cols - 1);
-    const int page = V.table[seq * V.table_stride + col];
-    return wanted && (unsigned)page < (unsigned)V.n_pages ? page : -1;
+    return V.table[seq * V.table_stride + col];
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
@@ -186,7 +190,7 @@ constexpr int RW = 4;       // waves
 constexpr int VPAD = 16;    // V rows in LDS: 16 elements of padding put 8 consecutive rows on different banks for the transposing reads
 
 template <int KIND, int DH>
-__global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void attend_rows_kernel(AttendP A) {
+__global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(AttendP A) {
     constexpr int NS = DH / 32;        // 32-dim slices of the score product
     constexpr int ND = DH / 16;        // 16-dim tiles of the output
     constexpr int VLD = DH + VPAD;
@@ -205,8 +209,8 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
     const int hk = (blockIdx.x / A.splits) % V.n_kv_heads, tile = blockIdx.x / A.splits / V.n_kv_heads;
     int seq, first;
     if (!find_tile(V, A.group, 16, tile, seq, first)) return;
-    const int row0 = kv_cu(V, seq), nq = kv_cu(V, seq + 1) - row0;
-    const int64_t p_base = (int64_t)V.kv_len[seq] - nq;  // position of the sequence's first row
+    const int row0 = scalar(kv_cu(V, seq)), nq = scalar(kv_cu(V, seq + 1)) - row0;
+    const int64_t p_base = (int64_t)scalar(V.kv_len[seq]) - nq;  // position of the sequence's first row
     const int n_tile = min(16, nq * A.group - first);
     // this lane's row; lanes behind the tile's end repeat its last row and store nothing
     const int row = first + min(fr, n_tile - 1);
@@ -233,10 +237,12 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
         float scale;
         unsigned dead;  // keys that no row sees, a bit each
     };
-    // page of key lane & 31 of step i
-    auto page_of = [&](int i) {
+    // key lane & 31 of step i: its table entry, and from that its page, -1 when no row of the tile can see it
+    auto entry_of = [&](int i) { return page_entry(V, seq, step_key<RS>(ks, i) + (lane & 31)); };
+    auto page_of = [&](int i, int entry) -> int {
         const int64_t j = step_key<RS>(ks, i) + (lane & 31);
-        return page_of_key(V, seq, j, i < i1 && j < ks.hi && !(A.window > 0 && j <= p_lo - A.window && j >= A.sinks));
+        const bool seen = (j < ks.hi) & !((A.window > 0) & (j <= p_lo - A.window) & (j >= A.sinks));
+        return seen & ((unsigned)entry < (unsigned)V.n_pages) ? entry : -1;
     };
     // (rows that are not there come from page 0 and are dropped later)
     auto load = [&](Step &x, int i, int page) {
@@ -329,7 +335,7 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
         for (int d = 0; d < ND; ++d) o[d] *= corr;
     };
     // one step; whole: every row sees every key of it.  x takes the next step's rows as soon as this one's are used.
-    int page = -1;
+    int entry = 0;  // of the step after next
     bool left = false;  // steps with values that are not finite and that some rows do not see: done at the end
     auto step = [&](Step &x, bool whole, int64_t key0, int next) {
         unsigned dead = x.dead;
@@ -345,8 +351,9 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
             __builtin_amdgcn_wave_barrier();
         }
         scores(x, s);
-        load(x, min(next, i1 - 1), page);
-        page = page_of(next + RW);
+        const int at = min(next, i1 - 1);
+        load(x, at, page_of(at, entry));
+        entry = entry_of(next + RW);
         softmax(s, whole ? ~0u : visible(dead, key0));
         // the residue of the probabilities' rounding goes through a second product: these kernels wait for memory, not for the MFMAs
         const u32x4 pb = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
@@ -364,8 +371,8 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
     };
     if (i0 < i1) {
         Step x;
-        load(x, i0, page_of(i0));
-        page = page_of(i0 + RW);
+        load(x, i0, page_of(i0, entry_of(i0)));
+        entry = entry_of(i0 + RW);
         auto whole = [&](int64_t key0) {
             return x.dead == 0 && key0 + RS - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + RS <= A.sinks);
         };
@@ -378,7 +385,7 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
 #pragma unroll 1
             for (int i = i0; i < i1; i += RW) {
                 const int64_t key0 = step_key<RS>(ks, i);
-                load(x, i, page_of(i));
+                load(x, i, page_of(i, entry_of(i)));
                 if (whole(key0) || !put(x, false)) continue;
                 const unsigned vis = visible(x.dead, key0);
                 float s[2][4];
@@ -460,18 +467,41 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : KIND == BF16 ? 2 : 3) void 
 // one step earlier still, a key per lane.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int CR = 128, CK = 64;  // rows, keys per step
+using gptr_t = const __attribute__((address_space(1))) void *;
+using lptr_t = __attribute__((address_space(3))) void *;
+// Asks the scheduler for an order of a block's LDS reads and products: AHEAD products' reads first (READS each), then a product and the
+// reads of the one AHEAD of it.  Left alone it reads a fragment, waits the whole LDS latency and multiplies.
+template <int PRODUCTS, int READS, int AHEAD> __device__ __forceinline__ void pipeline_reads() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < PRODUCTS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
 template <int KIND, int DH>
 __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_chunk_kernel(AttendP A) {
-    constexpr int KLD = DH + 8, VLD = DH + 16;  // row strides in LDS: fragment reads without bank conflicts
+    // Row strides in LDS.  8-bit rows pass through registers (their codes become bf16) and are padded; bf16 rows go to LDS
+    // directly, 1 KB a wave and load, which leaves no room for padding: the 16-byte pieces of a row are permuted instead.
+    constexpr bool DIRECT = KIND == BF16;
+    constexpr int KLD = DIRECT ? DH : DH + 8, VLD = DIRECT ? DH : DH + 16;
+    constexpr int ND = DH / 32;
     constexpr int EB = KIND == BF16 ? 2 : 1;
     constexpr int LPR = DH / 8, RPP = 256 / LPR, NP = CK / RPP;  // lanes per row, rows per pass, passes
     using raw_t = typename Raw<KIND>::type;
-    __shared__ __attribute__((aligned(16))) bf16_t kt[2][CK * KLD];
-    __shared__ __attribute__((aligned(16))) bf16_t vt[2][CK * VLD];
-    __shared__ __attribute__((aligned(16))) float sc[2][2][CK];
-    __shared__ int odd[2];  // a buffer whose values are not all finite
+    // (one object: the compiler waits for loads on their way to one shared array before it reads any other)
+    __shared__ __attribute__((aligned(1024))) struct {
+        bf16_t kt[2][CK * KLD], vt[2][CK * VLD];
+        float sc[2][2][CK];
+        int odd[2];  // the step whose values in a buffer are not all finite
+    } L;
+    auto &kt = L.kt;
+    auto &vt = L.vt;
+    auto &sc = L.sc;
+    auto &odd = L.odd;
     const KvView &V = A.V;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 31, h = lane >> 5;
     // tiles with the most keys first: in a chunk the later ones
@@ -479,8 +509,8 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
     const int split = rest % A.splits, tile = A.tiles - 1 - rest / A.splits;
     int seq, first;
     if (!find_tile(V, A.group, CR, tile, seq, first)) return;
-    const int row0 = kv_cu(V, seq), nq = kv_cu(V, seq + 1) - row0;
-    const int64_t p_base = (int64_t)V.kv_len[seq] - nq;
+    const int row0 = scalar(kv_cu(V, seq)), nq = scalar(kv_cu(V, seq + 1)) - row0;
+    const int64_t p_base = (int64_t)scalar(V.kv_len[seq]) - nq;
     const int n_tile = min(CR, nq * A.group - first);
     const int row = first + min(wave * 32 + fr, n_tile - 1);
     const int tok = row / A.group, head = hk * A.group + row % A.group;
@@ -502,32 +532,45 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     const int srow = tid / LPR, sub = tid % LPR;
-    // page of key `lane` of step i, -1 when no row of the tile can see it
-    auto page_of = [&](int i) -> int {
+    // key `lane` of step i: its table entry, and from that its page, -1 when no row of the tile can see it
+    auto entry_of = [&](int i) { return page_entry(V, seq, step_key<CK>(ks, i) + lane); };
+    auto page_of = [&](int i, int entry) -> int {
         const int64_t j = step_key<CK>(ks, i) + lane;
-        return page_of_key(V, seq, j, i < i1 && j < ks.hi && !(A.window > 0 && j <= p_lo - A.window && j >= A.sinks));
+        const bool seen = (j < ks.hi) & !((A.window > 0) & (j <= p_lo - A.window) & (j >= A.sinks));
+        return seen & ((unsigned)entry < (unsigned)V.n_pages) ? entry : -1;
     };
     // whether every row of the tile sees every key of the step at key0 (pages apart)
     auto all_see = [&](int64_t key0) { return key0 + CK - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + CK <= A.sinks); };
-    raw_t rk[NP], rv[NP];
+    // The piece (16 bytes) of row r that lies in slot s is s ^ turn(r): 16 rows' pieces of one dim lie on different banks (score
+    // products), and so do the 4 pieces of 8 rows that a transposing read takes.
+    auto turn = [](int r) { return DH == 128 ? (r & 3) << 2 | ((r >> 2) & 3) : ((r >> 1) & 1) << 2 | ((r >> 2) & 3); };
+    raw_t rk[DIRECT ? 1 : NP], rv[DIRECT ? 1 : NP];
     float rs = 0.0f;
-    const char *kbase = V.k + (hk * V.head_stride + sub * 8) * EB, *vbase = V.v + (hk * V.head_stride + sub * 8) * EB;
+    const int piece = DIRECT ? (lane % LPR) ^ turn(wave * (64 / LPR) + lane / LPR) : sub;  // (the same in every pass: rows 16 or 32 apart)
+    const char *kbase = V.k + (hk * V.head_stride + piece * 8) * EB, *vbase = V.v + (hk * V.head_stride + piece * 8) * EB;
     const float *sbase = (wave ? V.vs : V.ks) + hk * V.s_head;
-    // (rows that are not there come from page 0 and are dropped when they are stored)
-    auto load = [&](int64_t key0, int page) {
+    // rows of the step at key0 (those that are not there from page 0: they are dropped before they are used)
+    auto load = [&](int64_t key0, int page, int buf) {
         const int pg = max(page, 0), j = (int)(key0 + lane) & V.mask;
         const int64_t off = (pg * V.page_stride + j * V.row_stride) * EB;
 #pragma unroll
         for (int s = 0; s < NP; ++s) {
             const int64_t at = __shfl(off, s * RPP + srow);
-            rk[s] = *(const raw_t *)(kbase + at);
-            rv[s] = *(const raw_t *)(vbase + at);
+            if constexpr (DIRECT) {
+                const int row1 = s * RPP + wave * (64 / LPR);  // the wave's first row
+                __builtin_amdgcn_global_load_lds((gptr_t)(kbase + at), (lptr_t)&kt[buf][row1 * DH], 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((gptr_t)(vbase + at), (lptr_t)&vt[buf][row1 * DH], 16, 0, 0);
+            } else {
+                rk[s] = *(const raw_t *)(kbase + at);
+                rv[s] = *(const raw_t *)(vbase + at);
+            }
         }
-        if constexpr (KIND != BF16) {  // waves 0 and 1: the keys' and the values' scales, a key per lane
+        if constexpr (!DIRECT) {  // waves 0 and 1: the keys' and the values' scales, a key per lane
             if (wave < 2) rs = sbase[pg * V.s_page + j * V.s_row];
         }
     };
-    auto store = [&](int buf, bool check, unsigned long long gone) {
+    // 8-bit rows: registers -> LDS, keys that no row sees as zeros; mark: the step, if some row may not see some key of it
+    auto store = [&](int buf, int mark, unsigned long long gone) {
         bool bad = false;
 #pragma unroll
         for (int s = 0; s < NP; ++s) {
@@ -539,30 +582,51 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
 #pragma unroll
                 for (int q = 0; q < 4; ++q) x[q] = out ? 0 : x[q];
             }
-            if (KIND != INT8 && check) bad |= has_nonfinite(x);
+            if (KIND != INT8 && mark >= 0) bad |= has_nonfinite(x);
             *(u32x4 *)&vt[buf][r * VLD + sub * 8] = x;
         }
-        if constexpr (KIND != BF16) {
-            if (wave < 2) sc[buf][wave][lane] = rs;
-        }
-        if (KIND != INT8 && bad) odd[buf] = 1;
+        if (wave < 2) sc[buf][wave][lane] = rs;
+        if (KIND != INT8 && bad) odd[buf] = mark;
     };
-    if (tid < 2) odd[tid] = 0;
-    __syncthreads();
-    int page_n = page_of(i0);
-    unsigned long long dead = __ballot(page_n < 0), dead_n = 0;
+    // bf16 rows of a step that not every row sees whole: the same, done in LDS
+    auto mend = [&](int buf, int mark, unsigned long long gone) {
+        const int r = tid >> 2;
+        bf16_t *vr = &vt[buf][r * DH + (tid & 3) * (DH / 4)];
+        bool bad = false;
+#pragma unroll
+        for (int q = 0; q < DH / 32; ++q) {
+            if ((gone >> r) & 1) *(u32x4 *)(vr + 8 * q) = u32x4{0, 0, 0, 0};
+            else bad |= has_nonfinite(*(const u32x4 *)(vr + 8 * q));
+        }
+        if (bad) odd[buf] = mark;
+    };
+    // what is on its way to LDS is there, for every wave, and every wave is done with what it read before
+    auto arrived = [&]() {
+        if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    if (tid < 2) odd[tid] = -1;
+    int entry = 0;  // of the next step
+    unsigned long long dead = 0, dead_n = 0;
     if (i0 < i1) {
         const int64_t key0 = step_key<CK>(ks, i0);
-        load(key0, page_n);
-        page_n = page_of(i0 + 1);
-        store(0, !all_see(key0), dead);
+        const int page = page_of(i0, entry_of(i0));
+        dead = __ballot(page < 0);
+        load(key0, page, 0);
+        entry = entry_of(i0 + 1);
+        if constexpr (!DIRECT) {
+            __syncthreads();
+            store(0, all_see(key0) ? -1 : i0, dead);
+        }
     }
-    __syncthreads();
+    arrived();
     // s: weights of the values of a step, with the running maximum and sum.  MASKED: some row may not see some key of it, vis gets
     // the keys this lane's row sees; hide: none does
     auto weights = [&](auto masked, int cur, int64_t key0, bool hide, float (&s)[2][16], unsigned (&vis)[2]) {
         constexpr bool MASKED = decltype(masked)::value;
-        const bf16_t *kb = kt[cur];
+        // byte of row fr's first fragment; piece 2 c + h of a direct row is at slot (2 c + h) ^ turn(fr): an exclusive or with 32 c
+        const char *kb = (const char *)kt[cur] + fr * KLD * 2;
+        const int k0 = DIRECT ? (h ^ turn(fr)) * 16 : h * 16;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x16 a;
@@ -570,12 +634,13 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             for (int r = 0; r < 16; ++r) a[r] = 0.0f;
 #pragma unroll
             for (int c = 0; c < DH / 16; ++c) {
-                const u32x4 kf = *(const u32x4 *)(kb + (32 * t + fr) * KLD + 16 * c + 8 * h);
+                const u32x4 kf = *(const u32x4 *)(kb + 32 * t * KLD * 2 + (DIRECT ? k0 ^ (32 * c) : k0 + 32 * c));
                 a = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[c]), a, 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[t][r] = a[r];
         }
+        pipeline_reads<2 * (DH / 16), 1, 4>();
         if constexpr (KIND != BF16) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -644,54 +709,72 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         }
     };
     auto products = [&](int cur, const float (&s)[2][16]) {
-        const int gi = lane >> 4, ii = lane & 15;
-        const bf16_t *va = vt[cur] + (4 * h + (ii >> 2)) * VLD + 16 * (gi & 1) + (ii & 3) * 4;
+        const int gi = lane >> 4, ii = lane & 15, r0 = 4 * h + (ii >> 2), q0 = 2 * (gi & 1) + ((ii & 3) >> 1);
+        // byte of dims 32 d + .. of row 16 c + 8 e + r0: e and d turn the slot of a direct row by 32 e and 64 d bytes
+        const char *va = (const char *)vt[cur] + r0 * VLD * 2;
+        const int v0 = (DIRECT ? (q0 ^ turn(r0)) : q0) * 16 + (ii & 1) * 8;
+        auto fragments = [&](int c, u32x4 (&f)[ND]) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                u32x2 x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    x[e] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                         (lds_s16x4 *)(va + (16 * c + 8 * e) * VLD * 2 + (DIRECT ? v0 ^ (64 * d + 32 * e) : v0 + 64 * d))));
+                f[d] = u32x4{x[0].x, x[0].y, x[1].x, x[1].y};
+            }
+        };
+        u32x4 f[2][ND];
+        fragments(0, f[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            if (c < 3) fragments(c + 1, f[(c + 1) & 1]);
             const float *e = &s[c >> 1][8 * (c & 1)];
             const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
             u32x4 pl = {0, 0, 0, 0};
             if constexpr (KIND == INT8) pl = low_part(e, pb);  // (a code's scale leaves the largest weight no power of two: its rounding would show)
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d) {
-                const u32x2 a0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + 16 * c * VLD + 32 * d)));
-                const u32x2 a1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(va + (16 * c + 8) * VLD + 32 * d)));
-                const u32x4 a = {a0.x, a0.y, a1.x, a1.y};
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
+            for (int d = 0; d < ND; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[c & 1][d]), __builtin_bit_cast(bf16x8, pb), o[d], 0, 0, 0);
                 if constexpr (KIND == INT8)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[c & 1][d]), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
             }
         }
+        pipeline_reads<4 * ND, 2, ND>();
     };
     bool left = false;  // steps with values that are not finite and that some rows do not see: done at the end
     int i = i0, cur = 0;
-    // the next step's loads, this one, the next one's rows into the other buffer (last read before the previous barrier)
+    // the next step's rows on their way to the other buffer (last read before the previous barrier), this step
     auto advance = [&](auto masked) {
         const int64_t key0 = step_key<CK>(ks, i);
         const bool more = i + 1 < i1;
-        dead_n = __ballot(page_n < 0);
-        load(step_key<CK>(ks, more ? i + 1 : i), page_n);  // (behind the last step: loaded, not used)
-        page_n = page_of(i + 2);
+        const int64_t key1 = step_key<CK>(ks, more ? i + 1 : i);
+        if (more) {
+            const int page = page_of(i + 1, entry);
+            dead_n = __ballot(page < 0);
+            load(key1, page, cur ^ 1);
+            entry = entry_of(i + 2);
+        }
+        if constexpr (DIRECT && decltype(masked)::value) {
+            mend(cur, i, dead);
+            // (not __syncthreads, which would wait for the next step's rows as well)
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
         {
             float s[2][16];
             unsigned vis[2];
-            const bool hide = KIND != INT8 && decltype(masked)::value && odd[cur] != 0;
+            const bool hide = KIND != INT8 && decltype(masked)::value && odd[cur] == i;
             left |= hide;
             weights(masked, cur, key0, hide, s, vis);
             if (!hide) products(cur, s);
         }
-        const bool check = more && !all_see(step_key<CK>(ks, i + 1));
-        if (KIND != INT8) {
-            if (check) {
-                if (tid == 0) odd[cur ^ 1] = 0;
-                __syncthreads();
-            }
+        if constexpr (!DIRECT) {
+            if (more) store(cur ^ 1, all_see(key1) ? -1 : i + 1, dead_n);
         }
-        store(cur ^ 1, check, dead_n);
         dead = dead_n;
         cur ^= 1;
         ++i;
-        __syncthreads();
+        arrived();
     };
     // steps that every row sees whole run in a loop of their own: with the masks' code in it the compiler kept two copies of the
     // result and spilled
@@ -704,15 +787,15 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
 #pragma unroll 1
         for (i = i0; i < i1; ++i) {
             const int64_t key0 = step_key<CK>(ks, i);
-            const int pg = page_of(i);
+            const int pg = page_of(i, entry_of(i));
             dead = __ballot(pg < 0);
             if (dead == 0 && all_see(key0)) continue;
-            if (tid == 0) odd[0] = 0;
-            load(key0, pg);
+            load(key0, pg, 0);
+            arrived();
+            if constexpr (DIRECT) mend(0, i, dead);
+            else store(0, i, dead);
             __syncthreads();
-            store(0, true, dead);
-            __syncthreads();
-            if (odd[0] != 0) {
+            if (odd[0] == i) {
                 float s[2][16];
                 unsigned vis[2];
                 weights(std::true_type{}, 0, key0, false, s, vis);
@@ -724,12 +807,14 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
                     for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
                     const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
                     const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
-                    const bf16_t *vrow = vt[0] + k * VLD + 4 * h;
+                    const bf16_t *vrow = vt[0] + k * VLD;
 #pragma unroll
                     for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
-                            const float x = fmaf(pk, __uint_as_float((unsigned)vrow[32 * d + 8 * (q >> 2) + (q & 3)] << 16), o[d][q]);
+                            const int dim = 32 * d + 8 * (q >> 2) + 4 * h + (q & 3);
+                            const int at_dim = DIRECT ? ((dim >> 3) ^ turn(k)) * 8 + (dim & 7) : dim;
+                            const float x = fmaf(pk, __uint_as_float((unsigned)vrow[at_dim] << 16), o[d][q]);
                             o[d][q] = ok ? x : o[d][q];
                         }
                 }
