@@ -105,16 +105,24 @@ __device__ __forceinline__ bool has_nonfinite(u32x4 x) {  // of 8 bf16
 // in scalar registers.
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The tile of `tile_rows` rows a workgroup has: its sequence and the first row inside it.  Sequences are cut into tiles one
-// after the other; every wave looks through 64 sequences at a time.
-__device__ __forceinline__ bool find_tile(const KvView &V, int group, int tile_rows, int tile, int &seq, int &first_row) {
+// The tile of `tile_rows` rows (token, head of the group) a workgroup has.  Sequences are cut into tiles one after the other; every
+// wave looks through 64 sequences at a time, and each lane loads all that is to be known of its own: one trip to memory.
+struct Tile {
+    int seq, first;  // sequence, first row inside it
+    int row0, nq;    // the sequence's first row in q, its tokens
+    int kv_len;
+};
+__device__ __forceinline__ bool find_tile(const KvView &V, int group, int tile_rows, int tile, Tile &T) {
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int s0 = 0; s0 < V.n_seqs; s0 += 64) {
         const int b = s0 + lane;
-        int n = 0;
+        int n = 0, start = 0, end = 0, len = 0;
         if (b < V.n_seqs) {
-            const int64_t rows = (int64_t)max(0, kv_cu(V, b + 1) - kv_cu(V, b)) * group;
+            start = kv_cu(V, b);
+            end = kv_cu(V, b + 1);
+            len = V.kv_len[b];
+            const int64_t rows = (int64_t)max(0, end - start) * group;
             n = (int)((rows + tile_rows - 1) / tile_rows);
         }
         int incl = n;
@@ -127,8 +135,11 @@ __device__ __forceinline__ bool find_tile(const KvView &V, int group, int tile_r
         if (tile - base < all) {
             const unsigned long long m = __ballot(base + incl > tile);
             const int l = __ffsll((unsigned long long)m) - 1;
-            seq = scalar(s0 + l);
-            first_row = scalar((tile - base - __shfl(incl - n, l)) * tile_rows);
+            T.seq = scalar(s0 + l);
+            T.first = scalar((tile - base - __shfl(incl - n, l)) * tile_rows);
+            T.row0 = scalar(__shfl(start, l));
+            T.nq = scalar(__shfl(end, l)) - T.row0;
+            T.kv_len = scalar(__shfl(len, l));
             return true;
         }
         base += all;
@@ -176,15 +187,6 @@ __device__ __forceinline__ int page_entry(const KvView &V, int seq, int64_t j) {
 // Tiles of 16 rows: four waves take every fourth step of 32 keys; no wave waits for another before the end.  The next step's
 // rows are on their way while one is computed, their pages were looked up a step before (a key per lane).
 // ------------------------------------------------------------------------------------------------------------------------
-#ifndef ROWS_WANT
-#define ROWS_WANT 4
-#endif
-#ifndef CHUNK_WANT
-#define CHUNK_WANT 2
-#endif
-#ifndef ROWS_LEAST
-#define ROWS_LEAST 4
-#endif
 constexpr int RS = 32;      // keys per step
 constexpr int RW = 4;       // waves
 constexpr int VPAD = 16;    // V rows in LDS: 16 elements of padding put 8 consecutive rows on different banks for the transposing reads
@@ -207,10 +209,10 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, g = lane >> 4;
     const int split = blockIdx.x % A.splits;
     const int hk = (blockIdx.x / A.splits) % V.n_kv_heads, tile = blockIdx.x / A.splits / V.n_kv_heads;
-    int seq, first;
-    if (!find_tile(V, A.group, 16, tile, seq, first)) return;
-    const int row0 = scalar(kv_cu(V, seq)), nq = scalar(kv_cu(V, seq + 1)) - row0;
-    const int64_t p_base = (int64_t)scalar(V.kv_len[seq]) - nq;  // position of the sequence's first row
+    Tile T;
+    if (!find_tile(V, A.group, 16, tile, T)) return;
+    const int seq = T.seq, first = T.first, row0 = T.row0, nq = T.nq;
+    const int64_t p_base = (int64_t)T.kv_len - nq;  // position of the sequence's first row
     const int n_tile = min(16, nq * A.group - first);
     // this lane's row; lanes behind the tile's end repeat its last row and store nothing
     const int row = first + min(fr, n_tile - 1);
@@ -507,10 +509,10 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
     // tiles with the most keys first: in a chunk the later ones
     const int hk = blockIdx.x % V.n_kv_heads, rest = blockIdx.x / V.n_kv_heads;
     const int split = rest % A.splits, tile = A.tiles - 1 - rest / A.splits;
-    int seq, first;
-    if (!find_tile(V, A.group, CR, tile, seq, first)) return;
-    const int row0 = scalar(kv_cu(V, seq)), nq = scalar(kv_cu(V, seq + 1)) - row0;
-    const int64_t p_base = (int64_t)scalar(V.kv_len[seq]) - nq;
+    Tile T;
+    if (!find_tile(V, A.group, CR, tile, T)) return;
+    const int seq = T.seq, first = T.first, row0 = T.row0, nq = T.nq;
+    const int64_t p_base = (int64_t)T.kv_len - nq;
     const int n_tile = min(CR, nq * A.group - first);
     const int row = first + min(wave * 32 + fr, n_tile - 1);
     const int tok = row / A.group, head = hk * A.group + row % A.group;
@@ -840,17 +842,17 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
     if (part && h == 0) *(f32x2 *)(A.ws_ml + at * 2) = f32x2{m * A.c, l};
 }
 
-// Joins the splits of a row: one wave per (row, head).  Splits without keys have l = 0 and m = -inf.
+// Joins the splits of a row: one wave per (row, head).  Splits without keys have l = 0 and m = -inf.  Nothing here but latency
+// counts (a few hundred KB): a lane has four dims of every second (fourth) split, the loads of four of them at once.
 constexpr int MAX_SPLITS = 64;
 template <int DH>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendP A) {
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (item >= (int64_t)A.V.n_rows * A.n_heads) return;
-    const int t = (int)(item / A.n_heads), h = (int)(item % A.n_heads);
-    if (kv_seq_of_row(A.V, t) < 0) return;  // a row behind the last sequence
-    const int64_t step = (int64_t)A.V.n_rows * A.n_heads;
+__global__ __launch_bounds__(64) void attend_join_kernel(AttendP A) {
+    constexpr int LP = DH / 4, G = 64 / LP;  // lanes of a split's row, splits at a time
+    const int lane = threadIdx.x, d = lane % LP * 4, g = lane / LP;
+    const int t = blockIdx.x / A.n_heads, h = blockIdx.x % A.n_heads;
+    const int64_t item = blockIdx.x, step = (int64_t)A.V.n_rows * A.n_heads;
     float m = -INFINITY, l = 0.0f;
+    if (t < A.V.cu[0] || t >= A.V.cu[A.V.n_seqs]) return;  // a row of no sequence
     if (lane < A.splits) {
         const f32x2 x = *(const f32x2 *)(A.ws_ml + (item + lane * step) * 2);
         m = x.x;
@@ -859,17 +861,25 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendP A) {
     const float M = wave_max_desc(m);
     const float f = __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.0f : M));
     const float L = wave_sum_desc(l * f);
-    constexpr int E = DH / 64;
-    float acc[E] = {};
-    for (int s = 0; s < A.splits; ++s) {
-        const float fs = __shfl(f, s);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < A.splits; s0 += 4 * G) {
+        f32x4 x[4];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += fs * A.ws_o[(item + s * step) * DH + lane * E + e];
+        for (int i = 0; i < 4; ++i) x[i] = *(const f32x4 *)(A.ws_o + (item + min(s0 + i * G + g, A.splits - 1) * step) * DH + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * G + g;
+            const float fs = __shfl(f, s & 63);
+            const f32x4 y = acc + fs * x[i];
+            if (s < A.splits) acc = y;
+        }
     }
+#pragma unroll
+    for (int o = 32; o >= LP; o >>= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    bf16_t *op = A.out + t * A.o_row + h * A.o_head + lane * E;
-    if constexpr (E == 2) *(unsigned *)op = pack_bf16(acc[0] * inv, acc[1] * inv);
-    else *op = (bf16_t)(pack_bf16(acc[0] * inv, 0.0f) & 0xffffu);
+    if (g == 0) *(u32x2 *)(A.out + t * A.o_row + h * A.o_head + d) = u32x2{pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv)};
 }
 
 // How a call is cut up; the workspace and the launch agree because both ask here.
@@ -885,15 +895,21 @@ Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, in
     const bool chunk = (int64_t)longest * group > 48;
     p.rows = chunk ? CR : 16;
     p.tiles = (int64_t)b.n_rows * group / p.rows + b.n_seqs;
-    // workgroups of the tiles that hold rows when the sequences are as expected, keys of the longest
-    const int64_t expected = (int64_t)b.n_rows * group / p.rows + std::min(b.n_seqs, b.n_rows);
+    // workgroups of the tiles that hold rows when the sequences are as expected, steps of the longest
+    const int64_t seqs = std::min(b.n_seqs, b.n_rows);
+    const int64_t expected = std::min((int64_t)b.n_rows * group / p.rows + seqs, seqs * ceil_div<int64_t>((int64_t)longest * group, p.rows));
     const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
     int64_t keys = std::max(b.max_kv, 1);
     if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + sinks + std::min<int64_t>(longest, p.rows));
-    const int64_t steps = ceil_div<int64_t>(keys, chunk ? CK : RS), least = chunk ? 8 : ROWS_LEAST * RW;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((chunk ? CHUNK_WANT : ROWS_WANT) * (int64_t)n_cus / wgs, MAX_SPLITS));
-    p.steps = (int)std::max<int64_t>(ceil_div(steps, want), least);
-    p.splits = (int)std::max<int64_t>(1, ceil_div<int64_t>(steps, p.steps));
+    const int64_t steps = ceil_div<int64_t>(keys, chunk ? CK : RS), least = chunk ? 8 : 4 * RW;
+    // Workgroups a compute unit.  16-row tiles: three fit.  Under a window all have the same keys and one full round is best (32
+    // streams, 8 heads, window 2048: 33 us with three, 37 with four or more); without one the lengths differ, and more and shorter
+    // ones even out (8 streams of 9 - 33 k keys: 103 us with four, 94 with six, 93 with eight).  128-row tiles: two (8 prompts of 17 -
+    // 448 rows: 36 us with one to three, 42 with four: the partial results cost more than the shorter workgroups give).
+    const int64_t per_cu = chunk ? 2 : window > 0 ? 3 : 6;
+    const int64_t want = std::min<int64_t>(per_cu * n_cus / wgs, MAX_SPLITS);
+    p.splits = (int)std::max<int64_t>(1, std::min(want, steps / least));
+    p.steps = (int)ceil_div<int64_t>(steps, p.splits);
     return p;
 }
 size_t plan_bytes(const Plan &p, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads) {
@@ -951,9 +967,9 @@ void launch_kv_attend(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, con
 #undef KV_GO
     MW_HIP(hipGetLastError());
     if (p.splits > 1) {
-        const dim3 jg((unsigned)ceil_div<int64_t>((int64_t)b.n_rows * a.n_heads, 4));
-        if (c.head_dim == 64) hipLaunchKernelGGL(attend_join_kernel<64>, jg, dim3(256), 0, st, A);
-        else hipLaunchKernelGGL(attend_join_kernel<128>, jg, dim3(256), 0, st, A);
+        const dim3 jg((unsigned)((int64_t)b.n_rows * a.n_heads));
+        if (c.head_dim == 64) hipLaunchKernelGGL(attend_join_kernel<64>, jg, dim3(64), 0, st, A);
+        else hipLaunchKernelGGL(attend_join_kernel<128>, jg, dim3(64), 0, st, A);
         MW_HIP(hipGetLastError());
     }
 }
