@@ -909,7 +909,7 @@ class KvCache:
         (rows behind the last sequence are left as they are: in new ones their contents are undefined)."""
         d = self.device
         if out is None:
-            k, v = _torch.empty((2, n_rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=d)
+            k, v = _torch.empty((2, n_rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=d).unbind()
         else:
             k, v = out
         n = _rows(d, "out[0]", k, self.n_kv_heads, self.head_dim, dtype)
@@ -924,7 +924,7 @@ class KvCache:
         head_dim ** -0.5.  Rows behind the last sequence are left as they are (undefined without `out`).  The workspace
         is a tensor of the current stream's, or of the graph that captures the call."""
         d, bf16 = self.device, _torch.bfloat16
-        heads = q.shape[1]
+        heads = q.shape[1] if q.dim() > 1 else 0
         n, qr, qh = _rows(d, "q", q, heads, self.head_dim, bf16)
         if out is None:
             out = _torch.empty((n, heads, self.head_dim), dtype=bf16, device=d)

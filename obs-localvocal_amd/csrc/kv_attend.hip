@@ -28,6 +28,7 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
+using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 
@@ -95,10 +96,10 @@ __device__ __forceinline__ unsigned low_bits(int64_t n) {
     return c == 0 ? 0u : ~0u >> (32 - c);
 }
 __device__ __forceinline__ bool has_nonfinite(u32x4 x) {  // of 8 bf16
-    unsigned bad = 0;
+    u16x2 m = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (unsigned)((x[i] & 0x7f80u) == 0x7f80u) | (unsigned)((x[i] & 0x7f800000u) == 0x7f800000u);
-    return bad != 0;
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[i] & 0x7fff7fffu));
+    return max(m.x, m.y) >= 0x7f80;
 }
 
 // A value that is the same in all lanes, for the compiler to know: what follows from it (a step's keys, the loops' ends) then stays
@@ -185,7 +186,14 @@ __device__ __forceinline__ int page_entry(const KvView &V, int seq, int64_t j) {
 
 // ------------------------------------------------------------------------------------------------------------------------
 // Tiles of 16 rows: four waves take every fourth step of 32 keys; no wave waits for another before the end.  The next step's
-// rows are on their way while one is computed, their pages were looked up a step before (a key per lane).
+// rows are on their way while one is computed, their table entries were loaded a step before (a key per lane).
+//
+// Bound: HBM bytes of the keys and values, once the workgroups fill the card.  A lane loads 16 bytes (8-bit caches: two fragments'
+// worth, the dims permuted alike in q), 8 such loads in flight; rows go to LDS only for the transposing reads of V.  The step is one
+// body for whole and masked steps (two of them took 240 registers and a third of the waves), values that are not finite are left
+// to the end.  e4m3, 64 streams of 100 - 1500 keys, 20 heads of 64: 32.5 us, 4.3 TB/s (a copy reaches 4.7); int8, 8 streams of 9 - 33 k
+// keys, 32 heads on 8 of 128: 87 us, 4.1 TB/s, and 5 us for joining the splits; one stream of 224 keys: 6.5 us, launch and four
+// trips to memory one after the other (lengths, table, rows, result).
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int RS = 32;      // keys per step
 constexpr int RW = 4;       // waves
@@ -278,10 +286,17 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
                 if ((x.dead >> (16 * t + fr)) & 1) {
 #pragma unroll
                     for (int c = 0; c < NS; ++c) *row(t, c) = u32x4{0, 0, 0, 0};
-                } else if (KIND != INT8) {
-#pragma unroll
-                    for (int c = 0; c < NS; ++c) bad |= has_nonfinite(fragment<KIND>(x.v[t][c / FL], c % FL));
                 }
+            }
+        }
+        // (of a step that every row sees whole, too, where infinities can be: an infinity times a probability's residue is no number)
+        if (KIND == BF16 || (KIND == E4M3 && !whole)) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                bool odd = false;
+#pragma unroll
+                for (int c = 0; c < NS; ++c) odd |= has_nonfinite(fragment<KIND>(x.v[t][c / FL], c % FL));
+                bad |= odd & !((x.dead >> (16 * t + fr)) & 1);
             }
         }
         __builtin_amdgcn_wave_barrier();  // what other lanes of the wave read below is written above (LDS keeps a wave's order)
@@ -344,6 +359,7 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
         float s[2][4];
         if (put(x, whole)) {
             left = true;
+            whole = false;
             dead = ~0u;  // (as if no row saw it)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -388,7 +404,7 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
             for (int i = i0; i < i1; i += RW) {
                 const int64_t key0 = step_key<RS>(ks, i);
                 load(x, i, page_of(i, entry_of(i)));
-                if (whole(key0) || !put(x, false)) continue;
+                if (!put(x, whole(key0))) continue;
                 const unsigned vis = visible(x.dead, key0);
                 float s[2][4];
                 scores(x, s);
@@ -465,8 +481,13 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
 // 32 x 32 x 16 products: lane (row = l & 31, h = l >> 5) holds of a block of 32 keys the scores of keys 8 b + 4 h + r (b, r = 0 .. 3),
 // so a row's maximum and sum are completed by one exchange with lane ^ 32, and the probabilities of 16 keys are a fragment
 // of P^T if the contraction index is ordered (h, b, r) — the order two transposing reads give V^T in.
-// The next step's rows travel global -> registers -> LDS (8-bit codes become bf16 on the way); their pages are looked up
-// one step earlier still, a key per lane.
+// The next step's rows are on their way while one is computed: bf16 rows directly to LDS, 8-bit ones through registers (their codes
+// become bf16 there); their table entries are loaded one step earlier still, a key per lane.
+//
+// Bound: the issue of the softmax's 5 operations a score beside the matrix products (which alone keep a wave busy for 40 % of a
+// step), so two or three workgroups a compute unit, one's softmax under another's products.  2048 tokens behind 14336, 32 heads on
+// 8 of 128, bf16: 570 us, 0.91 PFLOP/s (a plain product of 8192 cubed reaches 1.38); with rows through registers and pages looked
+// up beside their loads it was 640.  8 prompts of 17 - 448 tokens, 20 heads of 64: 36 us, the longest tile's 23 steps.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int CR = 128, CK = 64;  // rows, keys per step
 using gptr_t = const __attribute__((address_space(1))) void *;
@@ -534,6 +555,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     const int srow = tid / LPR, sub = tid % LPR;
+    const bool busy = wave * 32 < n_tile;  // a wave without rows only loads
     // key `lane` of step i: its table entry, and from that its page, -1 when no row of the tile can see it
     auto entry_of = [&](int i) { return page_entry(V, seq, step_key<CK>(ks, i) + lane); };
     auto page_of = [&](int i, int entry) -> int {
@@ -762,11 +784,11 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             // (not __syncthreads, which would wait for the next step's rows as well)
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        {
+        const bool hide = KIND != INT8 && decltype(masked)::value && odd[cur] == i;
+        left |= hide;  // (in every wave: all of them load at the end)
+        if (busy) {
             float s[2][16];
             unsigned vis[2];
-            const bool hide = KIND != INT8 && decltype(masked)::value && odd[cur] == i;
-            left |= hide;
             weights(masked, cur, key0, hide, s, vis);
             if (!hide) products(cur, s);
         }
@@ -892,12 +914,17 @@ Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, in
     Plan p;
     const int group = n_heads / c.n_kv_heads;
     const int longest = b.max_rows > 0 ? std::min(b.max_rows, b.n_rows) : ceil_div(b.n_rows, b.n_seqs);
-    const bool chunk = (int64_t)longest * group > 48;
+    // Where several tiles of 16 rows, that read the keys again from L2, and one of 128, mostly empty, meet.  bf16, us with tiles of
+    // 16 / 128: 16 rows 22 / 20 and 42 / 54 (8 sequences of 1500 keys and 48 of 1000; 20 heads of 64), 32 rows 30 / 22 and 75 / 54.
+    // 8 bits, whose codes a 128-row tile converts for itself: 48 rows 26 / 32 and 58 / 82, 64 rows 30 / 33 and 70 / 82, 96 rows 33 / 37
+    // and 103 / 85 (e4m3); on 8 heads of 128 (int8) 48 rows 25 / 30 and 52 / 60, 64 rows 27 / 32 and 61 / 60, 96 rows 35 / 34 and 86 / 62.
+    const bool chunk = (int64_t)longest * group > (c.dtype == BF16 ? 16 : 64);
     p.rows = chunk ? CR : 16;
     p.tiles = (int64_t)b.n_rows * group / p.rows + b.n_seqs;
-    // workgroups of the tiles that hold rows when the sequences are as expected, steps of the longest
-    const int64_t seqs = std::min(b.n_seqs, b.n_rows);
-    const int64_t expected = std::min((int64_t)b.n_rows * group / p.rows + seqs, seqs * ceil_div<int64_t>((int64_t)longest * group, p.rows));
+    // workgroups of the tiles that hold rows when the sequences are as expected, steps of the longest.  (Not fewer than the rows
+    // fill: with a max_rows that is too small the splits, and the workspace, would grow with the rows.)
+    const int64_t seqs = std::min(b.n_seqs, b.n_rows), full = (int64_t)b.n_rows * group / p.rows;
+    const int64_t expected = std::max(full, std::min(full + seqs, seqs * ceil_div<int64_t>((int64_t)longest * group, p.rows)));
     const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
     int64_t keys = std::max(b.max_kv, 1);
     if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + sinks + std::min<int64_t>(longest, p.rows));

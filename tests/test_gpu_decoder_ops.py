@@ -388,6 +388,45 @@ def test_invisible_keys_and_values_may_hold_anything(pkg, kind, dim, q, kv, wind
         assert torch.isnan(got[q - 1]).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q", [1, 20])
+@pytest.mark.parametrize("at", [0, 37, 299])
+def test_an_infinite_value_that_is_seen(pkg, dim, q, at):
+    # every row that sees it: an infinity in its dims, the formula in the others; both signs in one dim are no number
+    c = Case(pkg, "bf16", dim, 2, 16, [q], [300 + q - 1])
+    inf = float("inf")
+    for j, d, x in ((at, 3, inf), (at, 17, -inf), (at, 40, inf), (150, 40, -inf)):
+        where = int(c.table[0, j // 16]), slice(None), j % 16, d
+        c.codes[1][where] = x
+        c.cache.v[where] = x
+    x = torch.randn(q, 4, dim, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    out = c.cache.attend(x, c.batch)
+    check_attend(c, x, out, dim ** -0.5)
+    out = out.cpu()
+    assert (out[:, :, 3] == inf).all() and (out[:, :, 17] == -inf).all() and torch.isnan(out[:, :, 40]).all()
+    rest = torch.ones(dim, dtype=torch.bool)
+    rest[[3, 17, 40]] = False
+    assert torch.isfinite(out[:, :, rest]).all()
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("max_rows,max_kv", [(0, 0), (1, 1), (1, 2**31 - 1), (2**31 - 1, 2**31 - 1), (500, 3)])
+def test_wrong_expectations_shape_the_launch_only(pkg, kind, max_rows, max_kv):
+    c = Case(pkg, kind, 64, 2, 16, [1, 200, 40], [900, 260, 40], extra_rows=300)
+    c.batch = pkg.KvBatch(*c.batch.tensors, max_rows, max_kv)
+    attend(c, 4)
+    attend(c, 4, window=70, sinks=5)
+
+
+def test_the_workspace_does_not_grow_with_wrong_expectations(pkg):
+    # the splits of a call are bounded by the rows it really has: 200000 of them leave no reason for any
+    import ctypes as C
+    c = Case(pkg, "bf16", 64, 2, 16, [1], [20])
+    for rows in (1, 0, 2**31 - 1):
+        b = pkg.KvBatch(*c.batch.tensors, rows, 2**31 - 1)._for(c.cache.device, 200000)
+        assert c.cache.L.mw_kv_attend_workspace(0, C.byref(c.cache.c), C.byref(b), 2, 0, 0) == 0
+
+
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("q", [1, 70])
 def test_large_scores(pkg, kind, q):
