@@ -486,8 +486,8 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
 //
 // Bound: the issue of the softmax's 5 operations a score beside the matrix products (which alone keep a wave busy for 40 % of a
 // step), so two or three workgroups a compute unit, one's softmax under another's products.  2048 tokens behind 14336, 32 heads on
-// 8 of 128, bf16: 570 us, 0.91 PFLOP/s (a plain product of 8192 cubed reaches 1.38); with rows through registers and pages looked
-// up beside their loads it was 640.  8 prompts of 17 - 448 tokens, 20 heads of 64: 36 us, the longest tile's 23 steps.
+// 8 of 128, bf16: 555 us, 0.93 PFLOP/s (a plain product of 8192 cubed reaches 1.38); with rows through registers and pages looked
+// up beside their loads it was 640.  One half's exponents under the other's products took more registers than there are.  8 prompts of 17 - 448 tokens, 20 heads of 64: 36 us, the longest tile's 23 steps.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int CR = 128, CK = 64;  // rows, keys per step
 using gptr_t = const __attribute__((address_space(1))) void *;
@@ -748,6 +748,9 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
                 f[d] = u32x4{x[0].x, x[0].y, x[1].x, x[1].y};
             }
         };
+        // a wave that multiplies goes before one at its softmax, which fills the gaps (570 -> 555 us; the scores' products raised as
+        // well, or the softmax instead: 565; for int8 the order it gives the code spills)
+        if constexpr (KIND == BF16) __builtin_amdgcn_s_setprio(1);
         u32x4 f[2][ND];
         fragments(0, f[0]);
 #pragma unroll
@@ -765,6 +768,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             }
         }
         pipeline_reads<4 * ND, 2, ND>();
+        if constexpr (KIND == BF16) __builtin_amdgcn_s_setprio(0);
     };
     bool left = false;  // steps with values that are not finite and that some rows do not see: done at the end
     int i = i0, cur = 0;

@@ -6,7 +6,8 @@
 //   int8  scale = max|x| / 127; code = rne(x / scale).  The quotient is not formed in fp32 (its rounding could carry a value
 //         over the half between two codes): the nearest whole number q of a product with the reciprocal is corrected by
 //         the remainder x - q scale, which fma gives exactly.
-// Bound: HBM bytes (each element is read once and written once), the launch when few rows are written.
+// Bound: HBM bytes (each element is read once and written once), the launch when few rows are written.  int8, 8 heads of 128, f32
+// rows: 9 k rows written in 31 us, 34 k read back in 80 (3.9 TB/s; a copy reaches 4.7); one row of 64 streams, 20 heads of 64, 4 us.
 #include "decoder_ops.hpp"
 
 namespace mw {
