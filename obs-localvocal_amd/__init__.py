@@ -933,6 +933,8 @@ class KvCache:
             no, o_r, o_h = _rows(d, "out", out, heads, self.head_dim, bf16)
             if no != n:
                 raise ValueError("out has another number of rows than q")
+        if window > 0x7fffffff or sinks > 0x7fffffff:  # (an int of C would take their low bits)
+            raise ValueError(f"window {window} and sinks {sinks} have to be below 2^31")
         b = C.byref(batch._for(d, n))
         need = self.L.mw_kv_attend_workspace(d.index, self._ref, b, heads, window, sinks)
         ws = _torch.empty(need, dtype=_torch.uint8, device=d) if need else None

@@ -410,6 +410,35 @@ def test_an_infinite_value_that_is_seen(pkg, dim, q, at):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("q", [1, 70])
+def test_lengths_beyond_the_table(pkg, kind, q):
+    # positions behind the table's columns hold nothing: the rows there see what the table has
+    c = Case(pkg, kind, 64, 2, 16, [q, q], [300, 90])
+    c.table = c.table[:, :7].contiguous()
+    c.batch = pkg.KvBatch(*c.batch.tensors[:2], c.table.cuda(), q, 300)
+    attend(c, 4)
+    attend(c, 4, window=40, sinks=5)
+    none = pkg.KvBatch(*c.batch.tensors[:2], c.table[:, :0].contiguous().cuda(), q, 300)
+    x = torch.randn(2 * q, 4, 64, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    assert (c.cache.attend(x, none) == 0).all()
+    assert all((t == 0).all() for t in c.cache.read(none, 2 * q, torch.float32))
+    before = c.cache.k.view(torch.uint8).clone()
+    c.cache.write(x[:, :2], x[:, 2:], none)
+    assert torch.equal(c.cache.k.view(torch.uint8), before)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_one_large_page_and_shared_pages(pkg, kind):
+    attend(Case(pkg, kind, 64, 1, 32768, [1, 60], [700, 600]), 2)
+    # two sequences with one prefix: the same pages named twice
+    c = Case(pkg, kind, 128, 2, 16, [1, 1, 40], [200, 200, 200])
+    c.table[1, :10] = c.table[0, :10]
+    c.table[2, :9] = c.table[0, :9]
+    c.batch = pkg.KvBatch(*c.batch.tensors[:2], c.table.cuda(), 40, 200)
+    attend(c, 4)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("max_rows,max_kv", [(0, 0), (1, 1), (1, 2**31 - 1), (2**31 - 1, 2**31 - 1), (500, 3)])
 def test_wrong_expectations_shape_the_launch_only(pkg, kind, max_rows, max_kv):
     c = Case(pkg, kind, 64, 2, 16, [1, 200, 40], [900, 260, 40], extra_rows=300)
@@ -740,6 +769,40 @@ def test_a_captured_step_replays(pkg):
         assert torch.equal(cache.k.view(torch.uint8), twin.k.view(torch.uint8))
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_captured_splits_and_cuts_replay(pkg, kind):
+    # the keys split over workgroups and joined, a chunk, and a sampler row that needs the histogram, in one graph; the second graph
+    # is captured while the first lives, and they are replayed in turn
+    c = Case(pkg, kind, 128, 2, 16, [1, 1], [4000, 3000])
+    d = Case(pkg, kind, 64, 2, 16, [90], [400])
+    g = torch.Generator().manual_seed(5)
+    q, r = torch.zeros(2, 8, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(90, 2, 64, dtype=torch.bfloat16, device="cuda")
+    x, u = torch.zeros(4, 30000, device="cuda"), torch.zeros(4, dtype=torch.float64, device="cuda")
+    k, p = torch.tensor([1000, 0, 800, 5], dtype=torch.int32).cuda(), torch.tensor([0.9, 0.8, 1.0, 0.5]).cuda()
+
+    def work():
+        return c.cache.attend(q, c.batch), d.cache.attend(r, d.batch), *pkg.sample_logits(x, u, top_k=k, top_p=p)
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        work()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, results = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(work())
+    for i in range(6):
+        for t in (q, r, x):
+            t.copy_(2 * torch.randn(t.shape, generator=g))
+        u.copy_(torch.rand(4, generator=g, dtype=torch.float64))
+        c.batch.tensors[1].copy_(torch.tensor([4000 - 600 * i, 3000 - 500 * i], dtype=torch.int32))
+        graphs[i & 1].replay()
+        want = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(results[i & 1], want)), i
+
+
 def test_two_streams_at_once(pkg):
     # the same cache read by calls that overlap: each has a workspace of its own
     c = Case(pkg, "bf16", 128, 4, 16, [1, 1, 1], [4000, 3500, 2000])
@@ -784,6 +847,14 @@ def test_refusals_on_the_gpu(pkg):
         c.cache.attend(torch.zeros(3 * 4 * 64 + 8, dtype=torch.bfloat16, device="cuda")[1:769].view(3, 4, 64), c.batch)
     with pytest.raises(ValueError):
         c.cache.attend(q, c.batch, out=q[:2])
+    for window, sinks in ((2**32 + 5, 0), (5, 2**31)):
+        with pytest.raises(ValueError, match="below 2"):
+            c.cache.attend(q, c.batch, window=window, sinks=sinks)
+    for window, sinks in ((-1, 0), (5, -1)):
+        with pytest.raises(RuntimeError, match="not negative"):
+            c.cache.attend(q, c.batch, window=window, sinks=sinks)
+    with pytest.raises(ValueError):
+        c.cache.attend(q.view(-1), c.batch)
     with pytest.raises(ValueError):
         c.cache.write(q[:, :2], q[:2, :2], c.batch)
     with pytest.raises(TypeError):
