@@ -476,7 +476,8 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// Tiles of 128 rows for chunks: four waves of 32 rows share steps of 64 keys, double-buffered in LDS.
+// Tiles of 128 rows for chunks: four waves of 32 rows share steps of 64 keys, double-buffered in LDS.  KW = 2: tiles of 64 rows, two
+// waves for the same 32, each with half of a step's keys; their results are joined at the end as splits are.
 //
 // 32 x 32 x 16 products: lane (row = l & 31, h = l >> 5) holds of a block of 32 keys the scores of keys 8 b + 4 h + r (b, r = 0 .. 3),
 // so a row's maximum and sum are completed by one exchange with lane ^ 32, and the probabilities of 16 keys are a fragment
@@ -487,7 +488,7 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
 // Bound: the issue of the softmax's 5 operations a score beside the matrix products (which alone keep a wave busy for 40 % of a
 // step), so two or three workgroups a compute unit, one's softmax under another's products.  2048 tokens behind 14336, 32 heads on
 // 8 of 128, bf16: 555 us, 0.93 PFLOP/s (a plain product of 8192 cubed reaches 1.38); with rows through registers and pages looked
-// up beside their loads it was 640.  One half's exponents under the other's products took more registers than there are.  8 prompts of 17 - 448 tokens, 20 heads of 64: 36 us, the longest tile's 23 steps.
+// up beside their loads it was 640.  One half's exponents under the other's products took more registers than there are.  8 prompts of 17 - 448 tokens, 20 heads of 64: 32 us (64-row tiles), the longest tile's 23 steps.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int CR = 128, CK = 64;  // rows, keys per step
 using gptr_t = const __attribute__((address_space(1))) void *;
@@ -505,12 +506,13 @@ template <int PRODUCTS, int READS, int AHEAD> __device__ __forceinline__ void pi
 }
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 
-template <int KIND, int DH>
+template <int KIND, int DH, int KW>
 __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_chunk_kernel(AttendP A) {
     // Row strides in LDS.  8-bit rows pass through registers (their codes become bf16) and are padded; bf16 rows go to LDS
     // directly, 1 KB a wave and load, which leaves no room for padding: the 16-byte pieces of a row are permuted instead.
     constexpr bool DIRECT = KIND == BF16;
     constexpr int KLD = DIRECT ? DH : DH + 8, VLD = DIRECT ? DH : DH + 16;
+    constexpr int ROWS = CR / KW, NT = 2 / KW;  // rows of the tile, blocks of 32 keys a wave has of a step
     constexpr int ND = DH / 32;
     constexpr int EB = KIND == BF16 ? 2 : 1;
     constexpr int LPR = DH / 8, RPP = 256 / LPR, NP = CK / RPP;  // lanes per row, rows per pass, passes
@@ -527,15 +529,16 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
     auto &odd = L.odd;
     const KvView &V = A.V;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 31, h = lane >> 5;
+    const int wr = KW == 1 ? wave : wave & 1, mine0 = KW == 1 ? 0 : (wave >> 1) * 32;  // the wave's rows (32 of them), its first key of a step
     // tiles with the most keys first: in a chunk the later ones
     const int hk = blockIdx.x % V.n_kv_heads, rest = blockIdx.x / V.n_kv_heads;
     const int split = rest % A.splits, tile = A.tiles - 1 - rest / A.splits;
     Tile T;
-    if (!find_tile(V, A.group, CR, tile, T)) return;
+    if (!find_tile(V, A.group, ROWS, tile, T)) return;
     const int seq = T.seq, first = T.first, row0 = T.row0, nq = T.nq;
     const int64_t p_base = (int64_t)T.kv_len - nq;
-    const int n_tile = min(CR, nq * A.group - first);
-    const int row = first + min(wave * 32 + fr, n_tile - 1);
+    const int n_tile = min(ROWS, nq * A.group - first);
+    const int row = first + min(wr * 32 + fr, n_tile - 1);
     const int tok = row / A.group, head = hk * A.group + row % A.group;
     const int64_t p = p_base + tok;
     const int64_t p_lo = p_base + first / A.group, p_hi = p_base + (first + n_tile - 1) / A.group;
@@ -555,7 +558,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     const int srow = tid / LPR, sub = tid % LPR;
-    const bool busy = wave * 32 < n_tile;  // a wave without rows only loads
+    const bool busy = wr * 32 < n_tile;  // a wave without rows only loads
     // key `lane` of step i: its table entry, and from that its page, -1 when no row of the tile can see it
     auto entry_of = [&](int i) { return page_entry(V, seq, step_key<CK>(ks, i) + lane); };
     auto page_of = [&](int i, int entry) -> int {
@@ -646,13 +649,13 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
     arrived();
     // s: weights of the values of a step, with the running maximum and sum.  MASKED: some row may not see some key of it, vis gets
     // the keys this lane's row sees; hide: none does
-    auto weights = [&](auto masked, int cur, int64_t key0, bool hide, float (&s)[2][16], unsigned (&vis)[2]) {
+    auto weights = [&](auto masked, int cur, int64_t key0, bool hide, float (&s)[NT][16], unsigned (&vis)[NT]) {
         constexpr bool MASKED = decltype(masked)::value;
         // byte of row fr's first fragment; piece 2 c + h of a direct row is at slot (2 c + h) ^ turn(fr): an exclusive or with 32 c
-        const char *kb = (const char *)kt[cur] + fr * KLD * 2;
+        const char *kb = (const char *)kt[cur] + (mine0 + fr) * KLD * 2;
         const int k0 = DIRECT ? (h ^ turn(fr)) * 16 : h * 16;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
             f32x16 a;
 #pragma unroll
             for (int r = 0; r < 16; ++r) a[r] = 0.0f;
@@ -664,22 +667,23 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[t][r] = a[r];
         }
-        pipeline_reads<2 * (DH / 16), 1, 4>();
+        pipeline_reads<NT * (DH / 16), 1, 4>();
         if constexpr (KIND != BF16) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const f32x4 f = *(const f32x4 *)&sc[cur][0][32 * t + 8 * b + 4 * h];
+                    const f32x4 f = *(const f32x4 *)&sc[cur][0][mine0 + 32 * t + 8 * b + 4 * h];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
                 }
         }
         if constexpr (MASKED) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                unsigned v = hide ? 0u : ~(unsigned)(dead >> (32 * t)) & low_bits(p - key0 + 1 - 32 * t);
-                if (A.window > 0) v &= ~low_bits(p - A.window - key0 + 1 - 32 * t) | low_bits((int64_t)A.sinks - key0 - 32 * t);
+            for (int t = 0; t < NT; ++t) {
+                const int64_t k1 = key0 + mine0 + 32 * t;
+                unsigned v = hide ? 0u : ~(unsigned)(dead >> (mine0 + 32 * t)) & low_bits(p - k1 + 1);
+                if (A.window > 0) v &= ~low_bits(p - A.window - k1 + 1) | low_bits((int64_t)A.sinks - k1);
                 vis[t] = v;
                 const unsigned mine = v >> (4 * h);
 #pragma unroll
@@ -689,7 +693,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         // running maximum (of the unscaled scores; the scale rides in the exponent's fma)
         float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
         mx = xor_max<32>(mx);
@@ -708,7 +712,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         const float ref = m == -INFINITY ? 0.0f : -m * A.c;
         float ps = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], A.c, ref));
@@ -717,25 +721,25 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         l += ps;
         if constexpr (KIND != BF16) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    const f32x4 f = *(const f32x4 *)&sc[cur][1][32 * t + 8 * b + 4 * h];
+                    const f32x4 f = *(const f32x4 *)&sc[cur][1][mine0 + 32 * t + 8 * b + 4 * h];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= f[r];
                 }
             if (MASKED) {  // (the scale of a value that is not seen may be anything)
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[t][r] = (vis[t] >> (4 * h)) & (1u << (8 * (r >> 2) + (r & 3))) ? s[t][r] : 0.0f;
             }
         }
     };
-    auto products = [&](int cur, const float (&s)[2][16]) {
+    auto products = [&](int cur, const float (&s)[NT][16]) {
         const int gi = lane >> 4, ii = lane & 15, r0 = 4 * h + (ii >> 2), q0 = 2 * (gi & 1) + ((ii & 3) >> 1);
         // byte of dims 32 d + .. of row 16 c + 8 e + r0: e and d turn the slot of a direct row by 32 e and 64 d bytes
-        const char *va = (const char *)vt[cur] + r0 * VLD * 2;
+        const char *va = (const char *)vt[cur] + (mine0 + r0) * VLD * 2;
         const int v0 = (DIRECT ? (q0 ^ turn(r0)) : q0) * 16 + (ii & 1) * 8;
         auto fragments = [&](int c, u32x4 (&f)[ND]) {
 #pragma unroll
@@ -754,8 +758,8 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         u32x4 f[2][ND];
         fragments(0, f[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (c < 3) fragments(c + 1, f[(c + 1) & 1]);
+        for (int c = 0; c < 2 * NT; ++c) {
+            if (c < 2 * NT - 1) fragments(c + 1, f[(c + 1) & 1]);
             const float *e = &s[c >> 1][8 * (c & 1)];
             const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
             u32x4 pl = {0, 0, 0, 0};
@@ -767,7 +771,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[c & 1][d]), __builtin_bit_cast(bf16x8, pl), o[d], 0, 0, 0);
             }
         }
-        pipeline_reads<4 * ND, 2, ND>();
+        pipeline_reads<2 * NT * ND, 2, ND>();
         if constexpr (KIND == BF16) __builtin_amdgcn_s_setprio(0);
     };
     bool left = false;  // steps with values that are not finite and that some rows do not see: done at the end
@@ -791,8 +795,8 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         const bool hide = KIND != INT8 && decltype(masked)::value && odd[cur] == i;
         left |= hide;  // (in every wave: all of them load at the end)
         if (busy) {
-            float s[2][16];
-            unsigned vis[2];
+            float s[NT][16];
+            unsigned vis[NT];
             weights(masked, cur, key0, hide, s, vis);
             if (!hide) products(cur, s);
         }
@@ -824,18 +828,18 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             else store(0, i, dead);
             __syncthreads();
             if (odd[0] == i) {
-                float s[2][16];
-                unsigned vis[2];
+                float s[NT][16];
+                unsigned vis[NT];
                 weights(std::true_type{}, 0, key0, false, s, vis);
 #pragma unroll 1
-                for (int k = 0; k < CK; ++k) {
-                    const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the 32 of its half
+                for (int k = 0; k < 32 * NT; ++k) {
+                    const int at = (k >> 5) * 16 + ((k >> 3) & 3) * 4 + (k & 3);  // the key among the wave's 16 NT of its half
                     float mine = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
+                    for (int e = 0; e < 16 * NT; ++e) mine = at == e ? s[e >> 4][e & 15] : mine;
                     const float other = __shfl_xor(mine, 32), pk = ((k >> 2) & 1) == h ? mine : other;
-                    const bool ok = ((k >> 5 ? vis[1] : vis[0]) >> (k & 31)) & 1;
-                    const bf16_t *vrow = vt[0] + k * VLD;
+                    const bool ok = (vis[NT == 1 ? 0 : k >> 5] >> (k & 31)) & 1;
+                    const bf16_t *vrow = vt[0] + (mine0 + k) * VLD;
 #pragma unroll
                     for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
@@ -851,7 +855,25 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         }
     }
     l += __shfl_xor(l, 32);
-    if (wave * 32 + fr >= n_tile) return;
+    if constexpr (KW == 2) {  // the two waves of the same rows: the second gives its part to the first (every wave is done with the rows in LDS)
+        float *x = (float *)&L + wr * 64 * (DH / 2 + 2) + lane;
+        if (mine0) {
+#pragma unroll
+            for (int e = 0; e < DH / 2; ++e) x[64 * e] = o[e >> 4][e & 15];
+            x[64 * (DH / 2)] = m;
+            x[64 * (DH / 2 + 1)] = l;
+        }
+        __syncthreads();
+        if (mine0) return;
+        const float m2 = x[64 * (DH / 2)], l2 = x[64 * (DH / 2 + 1)];
+        const float nm = fmaxf(m, m2), base = nm == -INFINITY ? 0.0f : nm;
+        const float f1 = __builtin_amdgcn_exp2f((m - base) * A.c), f2 = __builtin_amdgcn_exp2f((m2 - base) * A.c);
+#pragma unroll
+        for (int e = 0; e < DH / 2; ++e) o[e >> 4][e & 15] = o[e >> 4][e & 15] * f1 + x[64 * e] * f2;
+        l = l * f1 + l2 * f2;
+        m = nm;
+    }
+    if (wr * 32 + fr >= n_tile) return;
     const bool part = A.splits > 1;
     const float inv = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t at = ((int64_t)split * V.n_rows + row0 + tok) * A.n_heads + head;
@@ -918,25 +940,34 @@ Plan plan(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, int n_heads, in
     Plan p;
     const int group = n_heads / c.n_kv_heads;
     const int longest = b.max_rows > 0 ? std::min(b.max_rows, b.n_rows) : ceil_div(b.n_rows, b.n_seqs);
-    // Where several tiles of 16 rows, that read the keys again from L2, and one of 128, mostly empty, meet.  bf16, us with tiles of
-    // 16 / 128: 16 rows 22 / 20 and 42 / 54 (8 sequences of 1500 keys and 48 of 1000; 20 heads of 64), 32 rows 30 / 22 and 75 / 54.
-    // 8 bits, whose codes a 128-row tile converts for itself: 48 rows 26 / 32 and 58 / 82, 64 rows 30 / 33 and 70 / 82, 96 rows 33 / 37
-    // and 103 / 85 (e4m3); on 8 heads of 128 (int8) 48 rows 25 / 30 and 52 / 60, 64 rows 27 / 32 and 61 / 60, 96 rows 35 / 34 and 86 / 62.
-    const bool chunk = (int64_t)longest * group > (c.dtype == BF16 ? 16 : 64);
+    // Where several tiles of 16 rows, that read the keys again from L2, and one of 64 (bf16) or 128, mostly empty, meet.  bf16, us with
+    // tiles of 16 / 64: 16 rows 22 / 21 and 42 / 43 (8 sequences of 1500 keys and 48 of 1000; 20 heads of 64), 32 rows 30 / 21 and
+    // 75 / 43.  8 bits, whose codes a larger tile converts for itself, 16 / 128: 48 rows 26 / 32 and 58 / 82, 64 rows 30 / 33 and
+    // 70 / 82, 96 rows 33 / 37 and 103 / 85 (e4m3); on 8 heads of 128 (int8) 48 rows 25 / 30 and 52 / 60, 64 rows 27 / 32 and 61 / 60,
+    // 96 rows 35 / 34 and 86 / 62.
+    const int64_t rows = (int64_t)longest * group;
+    const bool chunk = rows > (c.dtype == BF16 ? 16 : 64);
+    // workgroups of the tiles that hold rows when the sequences are as expected.  (Not fewer than the rows fill: with a max_rows that
+    // is too small the splits, and the workspace, would grow with the rows.)
+    auto expected = [&](int tile) {
+        const int64_t seqs = std::min(b.n_seqs, b.n_rows), full = (int64_t)b.n_rows * group / tile;
+        return std::max<int64_t>(1, std::max(full, std::min(full + seqs, seqs * ceil_div<int64_t>(rows, tile))) * c.n_kv_heads);
+    };
     p.rows = chunk ? CR : 16;
+    // Tiles of 64 rows: the two waves of the same rows share the keys of a step, the chain of steps is half as long and the keys are
+    // read twice.  Where a tile of 128 is half empty anyway (64 rows, 48 sequences: 57 -> 47 us, on heads of 128 41 -> 36), and for heads
+    // of 64 where all fit at once (8 prompts of 17 - 448 rows: 36 -> 32 us; three chunks of 600 - 1777 rows, that do not: 34 -> 37; heads
+    // of 128, 96 and 128 rows: 26 -> 27, 29 -> 29; e4m3, whose codes are converted twice as well: 37 -> 43).
+    if (chunk && c.dtype == BF16 && (rows <= CR / 2 || (c.head_dim == 64 && expected(CR / 2) <= 3 * (int64_t)n_cus))) p.rows = CR / 2;
     p.tiles = (int64_t)b.n_rows * group / p.rows + b.n_seqs;
-    // workgroups of the tiles that hold rows when the sequences are as expected, steps of the longest.  (Not fewer than the rows
-    // fill: with a max_rows that is too small the splits, and the workspace, would grow with the rows.)
-    const int64_t seqs = std::min(b.n_seqs, b.n_rows), full = (int64_t)b.n_rows * group / p.rows;
-    const int64_t expected = std::max(full, std::min(full + seqs, seqs * ceil_div<int64_t>((int64_t)longest * group, p.rows)));
-    const int64_t wgs = std::max<int64_t>(1, expected * c.n_kv_heads);
+    const int64_t wgs = expected(p.rows);
     int64_t keys = std::max(b.max_kv, 1);
     if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + sinks + std::min<int64_t>(longest, p.rows));
     const int64_t steps = ceil_div<int64_t>(keys, chunk ? CK : RS), least = chunk ? 8 : 4 * RW;
     // Workgroups a compute unit.  16-row tiles: three fit.  Under a window all have the same keys and one full round is best (32
     // streams, 8 heads, window 2048: 33 us with three, 37 with four or more); without one the lengths differ, and more and shorter
-    // ones even out (8 streams of 9 - 33 k keys: 103 us with four, 94 with six, 93 with eight).  128-row tiles: two (8 prompts of 17 -
-    // 448 rows: 36 us with one to three, 42 with four: the partial results cost more than the shorter workgroups give).
+    // ones even out (8 streams of 9 - 33 k keys: 103 us with four, 94 with six, 93 with eight).  Chunks: two (8 prompts of 17 -
+    // 448 rows in tiles of 128: 36 us with one to three, 42 with four: partial results cost more than shorter workgroups give).
     const int64_t per_cu = chunk ? 2 : window > 0 ? 3 : 6;
     const int64_t want = std::min<int64_t>(per_cu * n_cus / wgs, MAX_SPLITS);
     p.splits = (int)std::max<int64_t>(1, std::min(want, steps / least));
@@ -983,7 +1014,8 @@ void launch_kv_attend(int n_cus, const mw_kv_cache &c, const mw_kv_batch &b, con
     const dim3 grid((unsigned)blocks), block(64 * RW);
 #define KV_GO(KIND, DH)                                                                            \
     do {                                                                                           \
-        if (p.rows == CR) hipLaunchKernelGGL((attend_chunk_kernel<KIND, DH>), grid, block, 0, st, A); \
+        if (p.rows == CR) hipLaunchKernelGGL((attend_chunk_kernel<KIND, DH, 1>), grid, block, 0, st, A); \
+        else if (KIND == BF16 && p.rows == CR / 2) hipLaunchKernelGGL((attend_chunk_kernel<BF16, DH, 2>), grid, block, 0, st, A); \
         else hipLaunchKernelGGL((attend_rows_kernel<KIND, DH>), grid, block, 0, st, A);              \
     } while (0)
 #define KV_DIM(KIND)                          \

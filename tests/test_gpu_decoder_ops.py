@@ -321,6 +321,17 @@ def test_chunks(pkg, kind, dim, hk, heads, page, q, kv):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 7)])
+def test_more_tiles_than_fit_at_once(pkg, kind, window, sinks):
+    # heads of 64 in tiles of 128 rows (fewer tiles, or fewer rows, take smaller ones); values that are not finite in the last tokens
+    c = Case(pkg, kind, 64, 64, 16, [130, 300, 270], [130, 600, 300])
+    for b, n in enumerate(c.kv):
+        c.cache.v[int(c.table[b, (n - 1) // 16]), :, (n - 1) % 16, 5] = float("inf") if kind == "bf16" else c.cache.v.new_zeros(())
+        c.codes[1][int(c.table[b, (n - 1) // 16]), :, (n - 1) % 16, 5] = float("inf") if kind == "bf16" else 0
+    attend(c, 64, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (33, 0), (64, 70), (100, 16), (1000, 3), (5000, 4), (7, 100000)])
 def test_windows_and_sinks(pkg, kind, window, sinks):
     attend(Case(pkg, kind, 128, 2, 16, [1, 1, 1, 1], [900, 65, 5, 1500]), 8, window=window, sinks=sinks)
