@@ -117,7 +117,7 @@ int mw_process_logits(struct whisper_context *ctx, const struct whisper_full_par
    page_size a power of two up to 32768, strides multiples of 16 bytes and bases 16-byte aligned.  Element types:
      MW_ELEM_BF16  no scales
      MW_ELEM_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| <= 448 scale
-     MW_ELEM_INT8  codes -127 .. 127; scale = max|x| / 127 (fp32), at least 2^-126
+     MW_ELEM_INT8  codes -127 .. 127; scale = max|x| * (1 / 127 rounded to fp32), at least 2^-126
    one fp32 scale per row and head, code = round to nearest even (x / scale).  A row of an 8-bit cache that holds an
    infinity or a NaN is kept as scale NaN and codes 0: it reads back as NaN. */
 enum mw_elem { MW_ELEM_F32 = 0, MW_ELEM_BF16 = 1, MW_ELEM_E4M3 = 2, MW_ELEM_INT8 = 3 };

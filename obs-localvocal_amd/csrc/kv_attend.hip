@@ -488,7 +488,8 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
 // Bound: the issue of the softmax's 5 operations a score beside the matrix products (which alone keep a wave busy for 40 % of a
 // step), so two or three workgroups a compute unit, one's softmax under another's products.  2048 tokens behind 14336, 32 heads on
 // 8 of 128, bf16: 555 us, 0.93 PFLOP/s (a plain product of 8192 cubed reaches 1.38); with rows through registers and pages looked
-// up beside their loads it was 640.  One half's exponents under the other's products took more registers than there are.  8 prompts of 17 - 448 tokens, 20 heads of 64: 32 us (64-row tiles), the longest tile's 23 steps.
+// up beside their loads it was 640.  One half's exponents under the other's products took more registers than there are.  8 prompts
+// of 17 - 448 tokens, 20 heads of 64: 32 us (64-row tiles), the longest tile's 23 steps.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int CR = 128, CK = 64;  // rows, keys per step
 using gptr_t = const __attribute__((address_space(1))) void *;

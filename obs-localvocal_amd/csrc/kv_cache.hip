@@ -3,7 +3,9 @@
 // A row of one head (64 or 128 elements) is held as bf16, or as 8-bit codes with one fp32 scale:
 //   e4m3  scale = the smallest power of two >= 2^-126 with max|x| <= 448 scale; x / scale is then exact (a shift of the
 //         exponent) and the code is the one rounding the format cannot do without
-//   int8  scale = max|x| / 127; code = rne(x / scale).  The quotient is not formed in fp32 (its rounding could carry a value
+//   int8  scale = max|x| x (1 / 127 rounded to fp32), what dividing a tensor by 127 on the GPU gives: a cache that a program fills by
+//         tensor operations holds the same bits (one row in 20 would have another last place, and a code in 10^7 would follow it).
+//         code = rne(x / scale).  The quotient is not formed in fp32 (its rounding could carry a value
 //         over the half between two codes): the nearest whole number q of a product with the reciprocal is corrected by
 //         the remainder x - q scale, which fma gives exactly.
 // Bound: HBM bytes (each element is read once and written once), the launch when few rows are written.  int8, 8 heads of 128, f32
@@ -143,7 +145,7 @@ template <int KIND, int DH, bool F32> __device__ __forceinline__ void write_row(
                 code.y = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[6] * inv, x[7] * inv, c, true);
             }
         } else {
-            scale = fmaxf(__uint_as_float(ub) / 127.0f, SCALE_MIN);
+            scale = fmaxf(__uint_as_float(ub) * (1.0f / 127.0f), SCALE_MIN);
             const float inv = 1.0f / scale;
             if (!bad) {
                 unsigned c[8];

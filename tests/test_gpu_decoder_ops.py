@@ -30,7 +30,7 @@ def quantise(kind, x):
     bad = ~torch.isfinite(x).all(-1)
     a = torch.where(bad, 0.0, amax).double()
     if kind == "int8":
-        s = torch.clamp((a.float() / 127), min=2.0 ** -126)
+        s = torch.clamp(a.float() * torch.tensor(1 / 127, dtype=torch.float32), min=2.0 ** -126)
         c = torch.round(x.double() / s.double()[..., None])
     else:
         m, e = torch.frexp(a)
@@ -236,6 +236,17 @@ def test_every_code_boundary(pkg, kind):
     codes, s = quantise(kind, x)
     want = (codes * s.double()[..., None]).float()
     assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), want.flip(0))
+
+
+def test_int8_scales_are_those_of_tensor_operations(pkg):
+    # the same bits as amax / 127 on the GPU, whose division by a constant is a product with its reciprocal
+    c = Case(pkg, "int8", 64, 4, 64, [2000], [2000])
+    x = torch.randn(2000, 4, 64, generator=torch.Generator().manual_seed(3)).cuda()
+    c.cache.write(x, x, c.batch)
+    s = x.abs().amax(-1) / 127
+    codes = torch.round(x.double() / s.double()[..., None])
+    got = c.cache.read(c.batch, 2000, torch.float32)[0]
+    assert torch.equal(got, codes.float() * s[..., None])
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
