@@ -252,7 +252,7 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
     auto page_of = [&](int i, int entry) -> int {
         const int64_t j = step_key<RS>(ks, i) + (lane & 31);
         const bool seen = (j < ks.hi) & !((A.window > 0) & (j <= p_lo - A.window) & (j >= A.sinks));
-        return seen & ((unsigned)entry < (unsigned)V.n_pages) ? entry : -1;
+        return (seen & ((unsigned)entry < (unsigned)V.n_pages)) ? entry : -1;
     };
     // (rows that are not there come from page 0 and are dropped later)
     auto load = [&](Step &x, int i, int page) {
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
     auto page_of = [&](int i, int entry) -> int {
         const int64_t j = step_key<CK>(ks, i) + lane;
         const bool seen = (j < ks.hi) & !((A.window > 0) & (j <= p_lo - A.window) & (j >= A.sinks));
-        return seen & ((unsigned)entry < (unsigned)V.n_pages) ? entry : -1;
+        return (seen & ((unsigned)entry < (unsigned)V.n_pages)) ? entry : -1;
     };
     // whether every row of the tile sees every key of the step at key0 (pages apart)
     auto all_see = [&](int64_t key0) { return key0 + CK - 1 <= p_lo && (A.window <= 0 || key0 > p_hi - A.window || key0 + CK <= A.sinks); };

@@ -321,20 +321,19 @@ template <bool BF> struct Source {
             }
         }
     }
-    // f(values, index of the first, round) over this thread's pieces, until it says false
+    // f(values, index of the first) over this thread's pieces in the order of the index
     template <typename F> __device__ __forceinline__ void pieces(F &&f) const {
         for (int k = 0; k < K; ++k) {
             float v[VEC];
             load(first(k), v);
-            if (!f(v, first(k), k)) break;
+            f(v, first(k));
         }
     }
     // f(value, index) over this thread's values in the order of the index
     template <typename F> __device__ __forceinline__ void each(F &&f) const {
-        pieces([&](const float (&v)[VEC], int i0, int) {
+        pieces([&](const float (&v)[VEC], int i0) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) f(v[e], i0 + e);
-            return true;
         });
     }
 };
@@ -360,7 +359,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
         if (threadIdx.x < SW) S.extra[threadIdx.x] = 0;
         __syncthreads();
         mine = 0.0;
-        src.pieces([&](const float (&v)[SRC::VEC], int i0, int) {
+        src.pieces([&](const float (&v)[SRC::VEC], int i0) {
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < SRC::VEC; ++e) {
@@ -377,7 +376,6 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
                 }
             }
             if (SUMS) mine += (double)sum;
-            return true;
         });
         __syncthreads();
         return S.n_list;
@@ -635,9 +633,8 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     };
     // (nothing dropped: the sums of the waves are those of step 2; after a cut they were formed on the way)
     const bool all_kept = !use_k && !use_p && !use_m && !greedy;
-    if (!all_kept && !have_sums) src.pieces([&](const float (&v)[VEC], int i0, int) {
+    if (!all_kept && !have_sums) src.pieces([&](const float (&v)[VEC], int i0) {
         mine += (double)piece_kept(v, i0);
-        return true;
     });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
