@@ -927,7 +927,7 @@ class KvCache:
         heads = q.shape[1] if q.dim() > 1 else 0
         n, qr, qh = _rows(d, "q", q, heads, self.head_dim, bf16)
         if out is None:
-            out = _torch.empty((n, heads, self.head_dim), dtype=bf16, device=d)
+            out = _torch.empty_like(q) if q.is_contiguous() else _torch.empty((n, heads, self.head_dim), dtype=bf16, device=d)
             o_r, o_h = heads * self.head_dim, self.head_dim
         else:
             no, o_r, o_h = _rows(d, "out", out, heads, self.head_dim, bf16)
