@@ -233,7 +233,7 @@ __device__ __forceinline__ u64 block_scan(Shared &S, u64 w, int n) {
 __device__ __forceinline__ u64 placed_key(u64 r, int place) { return (r >> 32) << 32 | (unsigned)r << 10 | (unsigned)place; }
 
 // The first bin whose running count (BY_COUNT: >= want) or running weight (>= want as doubles) is reached; bins follow each other in
-// the order of the tokens.  Results in S.found_*.
+// the order of the tokens.  Results in S.found_*; when no bin reaches it, found_bin is NB and found_count 0.
 template <bool BY_COUNT>
 __device__ void find_bin(Shared &S, const unsigned *cnt, const u64 *mass, unsigned base_cnt, u64 base_mass, double want) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -254,6 +254,10 @@ __device__ void find_bin(Shared &S, const unsigned *cnt, const u64 *mass, unsign
     if (lane == 63) {
         S.wave32[wave] = ci;
         S.wave64[wave] = mi;
+    }
+    if (t == 0) {
+        S.found_bin = NB;
+        S.found_count = 0;
     }
     __syncthreads();
     unsigned cb = base_cnt + ci - c[0] - c[1];
@@ -338,20 +342,22 @@ template <bool BF> struct Source {
     }
 };
 
-// The last kept token when the order is cut at `want` (a count or a weight): S.cut (its key) and S.cut_mass (weight up to and with it).
+// The last kept token when the order is cut at `want` (a count or a weight): S.cut (its key) and S.cut_mass (weight up to and with it);
+// false, and both as they were, when there is less than `want`.
 // On the way (SUMS) mine gets the thread's share of what is kept ahead of the list (tokens of at least `least`), S.extra what is kept of the
 // list for the wave that owns the token.
 template <bool BY_COUNT, bool SUMS, typename SRC>
-__device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R, double want, float least, double &mine) {
+__device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R, double want, float least, double &mine) {
     find_bin<BY_COUNT>(S, S.cnt, S.mass, 0, 0, want);
     const int bin = (int)S.found_bin;
+    if (bin == NB) return false;
     unsigned before = S.found_before;
     u64 before_mass = S.found_mass, lo = 0, hi = ~0ull;
-    const float top = (float)(-bin) / 64.0f, end = bin == NB - 1 ? -INFINITY : (float)(-bin - 1) / 64.0f;
-    auto in_bin = [&](float x) {
-        const float q = R.power(x);  // (64 q is exact)
-        return q > end && q <= top && x > -INFINITY;
-    };
+    // The bin's members, by the rule that counted them: a token far away (a mask of the type's lowest value) has a power of -inf and
+    // belongs to the last bin, a suppressed one to none.
+    const bool last_bin = bin == NB - 1;
+    const float top = (float)(-bin) / 64.0f, end = last_bin ? -INFINITY : (float)(-bin - 1) / 64.0f;
+    auto in_bin = [&](float q, float x) { return q <= top && (q > end || (last_bin && x > -INFINITY)); };  // (64 q is exact)
     // the bin's members with keys lo .. hi; returns how many there are (the list holds the first LIST that came)
     auto gather = [&]() -> unsigned {
         __syncthreads();
@@ -365,7 +371,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
             for (int e = 0; e < SRC::VEC; ++e) {
                 const float q = R.power(v[e]), w = SUMS ? __builtin_amdgcn_exp2f(q) : 0.0f;
                 if (SUMS) sum += q > top && w >= least ? w : 0.0f;
-                if (q > end && q <= top) {  // (few)
+                if (in_bin(q, v[e])) {  // (few)
                     const u64 r = rank_key(v[e], i0 + e);
                     if (r < lo) {
                         if (SUMS) sum += w >= least ? w : 0.0f;
@@ -389,7 +395,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
         __syncthreads();
         u64 a = ~0ull, b = 0;
         src.each([&](float x, int i) {
-            if (in_bin(x)) {
+            if (in_bin(R.power(x), x)) {
                 const u64 r = rank_key(x, i);
                 a = min(a, r);
                 b = max(b, r);
@@ -402,7 +408,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
         __syncthreads();
         lo = S.lo;
         hi = S.hi;
-        // keys are unique: a range divided down to single keys ends the loop at the latest
+        // keys are unique: a range divided down to single keys ends the loop at the latest, 2048 ways at a time after six rounds
         while (count > LIST) {
             int s = 0;
             while ((hi - lo) >> s >= NB) ++s;
@@ -412,7 +418,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
             }
             __syncthreads();
             src.each([&](float x, int i) {
-                if (in_bin(x)) {
+                if (in_bin(R.power(x), x)) {
                     const u64 r = rank_key(x, i);
                     if (r >= lo && r <= hi) {
                         const int b2 = (int)((r - lo) >> s);
@@ -423,6 +429,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
             });
             __syncthreads();
             find_bin<BY_COUNT>(S, S.cnt2, S.mass2, before, before_mass, want);
+            if (S.found_bin == NB) return false;
             before = S.found_before;
             before_mass = S.found_mass;
             count = S.found_count;
@@ -448,6 +455,7 @@ __device__ __forceinline__ void resolve(Shared &S, const SRC &src, const Row &R,
         if (SUMS && ahead && R.share(x) >= least) atomicAdd(&S.extra[src.owner((int)((unsigned)key >> 10))], R.weight(x));
     }
     __syncthreads();
+    return true;
 }
 
 template <bool BF>
@@ -594,6 +602,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     u64 cut = ~0ull;
     if (greedy) cut = (u64)(~ordered(mx)) << 32 | 0x7fffffffu;  // more equal largest logits than the list holds: the first of them is drawn
     double mine = 0.0;
+    bool have_sums = false;  // what each wave keeps is known from the last cut
     if (use_k || use_p) {
         if (lists) histogram();
         double kept = z * 0x1p31;
@@ -602,19 +611,20 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
             u64 live = S.cnt[2 * tid] + S.cnt[2 * tid + 1], t = 0;
             block_sum64(S, live, t);
             if ((u64)k < live) {
-                if (use_p) resolve<true, false>(S, src, R, (double)k, least, mine);
-                else resolve<true, true>(S, src, R, (double)k, least, mine);
-                cut = S.cut;
-                kept = (double)S.cut_mass;
+                const bool found = use_p ? resolve<true, false>(S, src, R, (double)k, least, mine) : resolve<true, true>(S, src, R, (double)k, least, mine);
+                if (found) {
+                    have_sums = !use_p;
+                    cut = S.cut;
+                    kept = (double)S.cut_mass;
+                }
             }
         }
         if (use_p) {
             __syncthreads();
-            resolve<false, true>(S, src, R, fmax((double)top_p * kept, 0.5), least, mine);
-            cut = S.cut;
+            have_sums = resolve<false, true>(S, src, R, fmax((double)top_p * kept, 0.5), least, mine);
+            if (have_sums) cut = S.cut;
         }
     }
-    const bool have_sums = (use_k || use_p) && cut != ~0ull;
 
     // ---- 4: draw ----
     const float cut_x = cut == ~0ull ? -INFINITY : key_value(cut);
@@ -633,9 +643,10 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     };
     // (nothing dropped: the sums of the waves are those of step 2; after a cut they were formed on the way)
     const bool all_kept = !use_k && !use_p && !use_m && !greedy;
-    if (!all_kept && !have_sums) src.pieces([&](const float (&v)[VEC], int i0) {
-        mine += (double)piece_kept(v, i0);
-    });
+    if (!all_kept && !have_sums) {
+        mine = 0.0;
+        src.pieces([&](const float (&v)[VEC], int i0) { mine += (double)piece_kept(v, i0); });
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
     __syncthreads();
