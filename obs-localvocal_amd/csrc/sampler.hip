@@ -353,11 +353,15 @@ __device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R,
     if (bin == NB) return false;
     unsigned before = S.found_before;
     u64 before_mass = S.found_mass, lo = 0, hi = ~0ull;
-    // The bin's members, by the rule that counted them: a token far away (a mask of the type's lowest value) has a power of -inf and
-    // belongs to the last bin, a suppressed one to none.
-    const bool last_bin = bin == NB - 1;
-    const float top = (float)(-bin) / 64.0f, end = last_bin ? -INFINITY : (float)(-bin - 1) / 64.0f;
-    auto in_bin = [&](float q, float x) { return q <= top && (q > end || (last_bin && x > -INFINITY)); };  // (64 q is exact)
+    // The bin's members by the rule that counted them, end <= q <= top (64 q is exact; one end is the next number above -(bin + 1) / 64).
+    // The last bin goes down to -inf: a token far away (a mask of the type's lowest value) has that power and belongs to it, a
+    // suppressed one has it too and belongs to none.  (The test of x stands behind those of q, which few pass: in one expression 256 rows of
+    // 128 000 took 82 us instead of 78.)
+    const float top = (float)(-bin) / 64.0f, end = bin == NB - 1 ? -INFINITY : __uint_as_float(__float_as_uint((float)(-bin - 1) / 64.0f) - 1);
+    auto in_bin = [&](float x) {
+        const float q = R.power(x);
+        return q >= end && q <= top && x > -INFINITY;
+    };
     // the bin's members with keys lo .. hi; returns how many there are (the list holds the first LIST that came)
     auto gather = [&]() -> unsigned {
         __syncthreads();
@@ -371,8 +375,9 @@ __device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R,
             for (int e = 0; e < SRC::VEC; ++e) {
                 const float q = R.power(v[e]), w = SUMS ? __builtin_amdgcn_exp2f(q) : 0.0f;
                 if (SUMS) sum += q > top && w >= least ? w : 0.0f;
-                if (in_bin(q, v[e])) {  // (few)
+                if (q >= end && q <= top) {  // (few)
                     const u64 r = rank_key(v[e], i0 + e);
+                    if (!(v[e] > -INFINITY)) continue;
                     if (r < lo) {
                         if (SUMS) sum += w >= least ? w : 0.0f;
                     } else if (r <= hi) {
@@ -395,7 +400,7 @@ __device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R,
         __syncthreads();
         u64 a = ~0ull, b = 0;
         src.each([&](float x, int i) {
-            if (in_bin(R.power(x), x)) {
+            if (in_bin(x)) {
                 const u64 r = rank_key(x, i);
                 a = min(a, r);
                 b = max(b, r);
@@ -418,7 +423,7 @@ __device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R,
             }
             __syncthreads();
             src.each([&](float x, int i) {
-                if (in_bin(R.power(x), x)) {
+                if (in_bin(x)) {
                     const u64 r = rank_key(x, i);
                     if (r >= lo && r <= hi) {
                         const int b2 = (int)((r - lo) >> s);
