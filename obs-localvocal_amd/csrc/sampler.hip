@@ -107,15 +107,16 @@ __device__ __forceinline__ int block_count(Shared &S, bool yes) {
     for (int w = 0; w < SW; ++w) t += (int)S.wave32[w];
     return t;
 }
-// v summed over the workgroup in one order (fp32 inside a wave, 64 bits over the waves); every thread gets the sum
-__device__ __forceinline__ double block_sum_f(Shared &S, float v) {
-    v = wave_sum_desc(v);
+// v summed over the workgroup in one order; every thread gets the sum, S.wave_d the waves' parts
+__device__ __forceinline__ double block_sum_d(Shared &S, double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) S.wave_f[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) S.wave_d[threadIdx.x >> 6] = v;
     __syncthreads();
     double t = 0.0;
 #pragma unroll
-    for (int w = 0; w < SW; ++w) t += (double)S.wave_f[w];
+    for (int w = 0; w < SW; ++w) t += S.wave_d[w];
     return t;
 }
 // A value that at least `want` of the threads' largest values reach, and not many more: bisection between the row's maximum and
@@ -500,7 +501,9 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     else if (use_m && !use_p) bound = mx + (__builtin_amdgcn_logf(least) - 1e-5f) / R.c;  // (log2; a little more than what is kept)
     bound = fmaxf(bound, -3.4028235e38f);  // (-inf is never listed)
     const bool lists = bound < INFINITY;
-    float zf = 0.0f;
+    // the thread's sum: fp32 inside 16 bytes of a row, 64 bits over them (in fp32 a long row of equal small weights was off by 3e-6)
+    double zd = 0.0;
+    constexpr int VEC = Source<BF>::VEC;
     // histogram over 64 d: counts if top-k asks for them, weights if top-p does.  The last bin takes all that is far away: in
     // registers first, or its one address would be waited for by every lane.
     auto histogram = [&]() {
@@ -511,18 +514,23 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
         __syncthreads();
         unsigned far = 0;
         u64 far_mass = 0;
-        src.each([&](float x, int) {
-            const float q = R.power(x), w = __builtin_amdgcn_exp2f(q);
-            zf += w;
-            const unsigned w32 = (unsigned)fmaf(w, 2147483648.0f, 0.5f);
-            if (q > -(float)(NB - 1) / 64.0f) {
-                const int b = (int)(-64.0f * q);
-                if (use_k) atomicAdd(&S.cnt[b], 1u);
-                if (use_p) atomicAdd(&S.mass[b], (u64)w32);
-            } else if (x > -INFINITY) {
-                ++far;
-                far_mass += w32;
+        src.pieces([&](const float (&v)[VEC], int) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float q = R.power(v[e]), w = __builtin_amdgcn_exp2f(q);
+                sum += w;
+                const unsigned w32 = (unsigned)fmaf(w, 2147483648.0f, 0.5f);
+                if (q > -(float)(NB - 1) / 64.0f) {
+                    const int b = (int)(-64.0f * q);
+                    if (use_k) atomicAdd(&S.cnt[b], 1u);
+                    if (use_p) atomicAdd(&S.mass[b], (u64)w32);
+                } else if (v[e] > -INFINITY) {
+                    ++far;
+                    far_mass += w32;
+                }
             }
+            zd += (double)sum;
         });
         if (far) {
             atomicAdd(&S.cnt[NB - 1], far);
@@ -531,19 +539,29 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
         __syncthreads();
     };
     if (lists) {
-        src.each([&](float x, int i) {
-            zf += R.share(x);
-            if (x >= bound) {
-                const unsigned at = atomicAdd(&S.n_list, 1u);
-                if (at < LIST) S.list_r[at] = rank_key(x, i);
+        src.pieces([&](const float (&v)[VEC], int i0) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                sum += R.share(v[e]);
+                if (v[e] >= bound) {
+                    const unsigned at = atomicAdd(&S.n_list, 1u);
+                    if (at < LIST) S.list_r[at] = rank_key(v[e], i0 + e);
+                }
             }
+            zd += (double)sum;
         });
     } else if (use_k || use_p) {
         histogram();
     } else {
-        src.each([&](float x, int) { zf += R.share(x); });
+        src.pieces([&](const float (&v)[VEC], int) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += R.share(v[e]);
+            zd += (double)sum;
+        });
     }
-    const double z = block_sum_f(S, zf);
+    const double z = block_sum_d(S, zd);
     // a NaN anywhere is one in the sum; with a maximum of +inf or -inf nothing can be drawn
     if (z != z || !(mx < INFINITY) || mx == -INFINITY || temp != temp || top_p != top_p || min_p != min_p || u != u) {
         if (tid == 0) {
@@ -634,7 +652,6 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     // ---- 4: draw ----
     const float cut_x = cut == ~0ull ? -INFINITY : key_value(cut);
     const int cut_i = cut == ~0ull ? 0x7fffffff : (int)(unsigned)cut;
-    constexpr int VEC = Source<BF>::VEC;
     auto weight_kept = [&](float x, int i) -> float {
         const float w = R.share(x);
         const bool keep = x > cut_x || (x == cut_x && i <= cut_i);
@@ -655,7 +672,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
     __syncthreads();
-    if (lane == 0) S.wave_d[wave] = all_kept ? (double)S.wave_f[wave] : have_sums ? mine + (double)S.extra[wave] * 0x1p-40 : mine;
+    if (lane == 0) S.wave_d[wave] = all_kept ? S.wave_d[wave] : have_sums ? mine + (double)S.extra[wave] * 0x1p-40 : mine;
     __syncthreads();
     double total = 0.0;
 #pragma unroll

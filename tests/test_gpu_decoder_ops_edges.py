@@ -41,3 +41,17 @@ def test_rows_with_masks_do_not_depend_on_their_neighbours(pkg):
         one, lp = pkg.sample_logits(x[r:r + 1], u[r:r + 1].cuda(), *(a[r:r + 1].cuda() for a in (t, k, p)))
         assert one.item() == ids[r].item() and lp.item() == lps[r].item(), r
     check_sample(pkg, x, u, t.tolist(), k.tolist(), p.tolist())
+
+
+@pytest.mark.parametrize("vocab", [51866, 1 << 20])
+@pytest.mark.parametrize("depth", [9.3, 12.7, 15.0])
+def test_sums_over_long_flat_tails(pkg, vocab, depth):
+    # many equal small weights: the roundings of a running sum all have one sign
+    x = torch.full((6, vocab), -depth)
+    x[:, vocab // 3] = 0.0
+    x[3:, ::3] -= 0.7
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.9, 1 - 2.0 ** -53], dtype=torch.float64)
+    check_sample(pkg, x.cuda(), u)
+    check_sample(pkg, x.cuda(), u, t=[0.9, 1.0, 1.2] * 2)
+    check_sample(pkg, x.cuda(), u, m=[1e-9])
+    check_sample(pkg, x.cuda(), u, k=[vocab - 5])
