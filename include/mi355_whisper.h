@@ -164,7 +164,7 @@ int mw_kv_attend_device(int device, void *stream, const struct mw_kv_cache *cach
                         int64_t out_head_stride, float scale, int window, int sinks, void *workspace, size_t workspace_bytes);
 /* One token per row of logits (MW_ELEM_F32 or MW_ELEM_BF16, [n_rows] rows row_stride elements apart).  x = logit / temperature[row];
    the tokens in the order (x falling, index rising); top_k keeps that many of them; top_p, of those, the fewest that hold
-   at least top_p of their probability; min_p, of those, the ones at least min_p times as likely as the likeliest; the token
+   at least top_p of their probability (counted in 2^-43 of the likeliest token's); min_p, of those, the ones at least min_p times as likely as the likeliest; the token
    is the first in the order of the index whose cumulated probability reaches u[row] (0 <= u < 1) of what is kept.
    temperature <= 0: the first largest logit.  top_k <= 0, top_p >= 1 and min_p <= 0 keep all; the likeliest token is always
    kept.  The settings are device arrays [n_rows], each may be null (temperature 1, nothing dropped).  logprobs (may be null)

@@ -56,7 +56,13 @@ struct Row {
     // -d = (x - max) log2(e) / temperature; -inf stays -inf.  Both roundings keep the order of the tokens.
     __device__ __forceinline__ float power(float x) const { return (x - max) * c; }
     __device__ __forceinline__ float share(float x) const { return __builtin_amdgcn_exp2f(power(x)); }  // of the likeliest token's probability
-    __device__ __forceinline__ unsigned weight32(float x) const { return (unsigned)fmaf(share(x), 2147483648.0f, 0.5f); }  // 2^31 of it, to the nearest
+    // 2^43 of a share, to the nearest: 2^20 of them fit in 64 bits, and what 2^20 tokens of less than half a unit leave out is 2^-24 of the
+    // likeliest one's (with 2^31 units top-p did not see tails that it has to cut)
+    static __device__ __forceinline__ u64 units(float share) {
+        const float f = fmaf(share, 8796093022208.0f, 0.5f);
+        const unsigned hi = (unsigned)(f * 2.3283064365386963e-10f);  // 2^-32
+        return (u64)hi << 32 | (unsigned)fmaf((float)hi, -4294967296.0f, f);
+    }
     // floor(2^(40 - d)), from d in 64 bits: 2^-d = 2^-whole 2^-part, |part| <= 1/2
     __device__ __forceinline__ u64 weight(float x) const {
         const double d = fmin(((double)max - (double)x) * c_d, 200.0), w = rint(d);
@@ -429,7 +435,7 @@ __device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R,
                     if (r >= lo && r <= hi) {
                         const int b2 = (int)((r - lo) >> s);
                         atomicAdd(&S.cnt2[b2], 1u);
-                        atomicAdd(&S.mass2[b2], (u64)R.weight32(x));
+                        atomicAdd(&S.mass2[b2], Row::units(R.share(x)));
                     }
                 }
             });
@@ -449,7 +455,7 @@ __device__ __forceinline__ bool resolve(Shared &S, const SRC &src, const Row &R,
     const int n = (int)min(S.n_list, (unsigned)LIST), tid = threadIdx.x;
     const u64 key = block_sort(S, tid < n ? placed_key(S.list_r[tid], tid) : ~0ull, n);
     const float x = key_value(key);
-    const u64 w = tid < n ? R.weight32(x) : 0;
+    const u64 w = tid < n ? Row::units(R.share(x)) : 0;
     const u64 mass = before_mass + block_scan(S, w, n);
     if (tid < n) {
         const bool ahead = BY_COUNT ? (double)(before + tid) < want : (double)(mass - w) < want;
@@ -520,14 +526,14 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
             for (int e = 0; e < VEC; ++e) {
                 const float q = R.power(v[e]), w = __builtin_amdgcn_exp2f(q);
                 sum += w;
-                const unsigned w32 = (unsigned)fmaf(w, 2147483648.0f, 0.5f);
+                const u64 un = Row::units(w);  // (ahead of the branch: inside it 256 rows of 128 000 took 84 us, not 80)
                 if (q > -(float)(NB - 1) / 64.0f) {
                     const int b = (int)(-64.0f * q);
                     if (use_k) atomicAdd(&S.cnt[b], 1u);
-                    if (use_p) atomicAdd(&S.mass[b], (u64)w32);
+                    if (use_p) atomicAdd(&S.mass[b], un);
                 } else if (v[e] > -INFINITY) {
                     ++far;
-                    far_mass += w32;
+                    far_mass += un;
                 }
             }
             zd += (double)sum;
@@ -596,13 +602,9 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
         bool keep = tid < n && (!use_k || tid < k);
         if (use_p) {
             const u64 wt = tid < n ? S.list_w[key & (LIST - 1)] : 0, upto = block_scan(S, wt, n);
-            double kept = z * 0x1p40;
-            if (use_k) {
-                if (tid == min(k, n) - 1) S.kept = upto;
-                __syncthreads();
-                kept = (double)S.kept;
-            }
-            keep &= tid == 0 || (double)(upto - wt) < (double)top_p * kept;
+            if (tid == min(k, n) - 1) S.kept = upto;  // (a list without top-k has no top-p either)
+            __syncthreads();
+            keep &= tid == 0 || (double)(upto - wt) < (double)top_p * (double)S.kept;
         }
         keep &= R.share(x) >= least;
         const int nk = block_count(S, keep);
@@ -628,11 +630,12 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
     bool have_sums = false;  // what each wave keeps is known from the last cut
     if (use_k || use_p) {
         if (lists) histogram();
-        double kept = z * 0x1p31;
+        // what there is by the histogram's own sums: top-p's share of any other total could be more than its bins hold
+        u64 live = S.cnt[2 * tid] + S.cnt[2 * tid + 1], mass = S.mass[2 * tid] + S.mass[2 * tid + 1];
+        block_sum64(S, live, mass);
+        double kept = (double)mass;
         if (use_k) {
             // fewer tokens than k may be left by the suppressed ones: nothing to cut then
-            u64 live = S.cnt[2 * tid] + S.cnt[2 * tid + 1], t = 0;
-            block_sum64(S, live, t);
             if ((u64)k < live) {
                 const bool found = use_p ? resolve<true, false>(S, src, R, (double)k, least, mine) : resolve<true, true>(S, src, R, (double)k, least, mine);
                 if (found) {

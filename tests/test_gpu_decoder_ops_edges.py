@@ -1,9 +1,10 @@
 """GPU: the sampler and the attention at the edges of what their arguments allow, against the plain forms (and under the
 tolerances) of test_gpu_decoder_ops.py."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_decoder_ops import check_sample
+from test_gpu_decoder_ops import check_sample, sample_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,56 @@ def test_sums_over_long_flat_tails(pkg, vocab, depth):
     check_sample(pkg, x.cuda(), u, t=[0.9, 1.0, 1.2] * 2)
     check_sample(pkg, x.cuda(), u, m=[1e-9])
     check_sample(pkg, x.cuda(), u, k=[vocab - 5])
+
+
+def check_cut(pkg, logits, u, p, k=(0,), t=(1.0,), m=(0.0,)):
+    """check_sample where many tokens lie so near to the cut of top_p that its place among them is a matter of roundings.  What is asked
+    for and what runs up to it are each off by 2^-22 of the weight, which moves the cut over 2^-21 of it; the token has to be
+    one that top_p + 2^-21 keeps.  A cumulated share moves with the tokens beside the cut (2^-21), with the total (2^-21) and by
+    the 2^-21 of check_sample: 2^-19 holds them."""
+    rows = logits.shape[0]
+    on = lambda a, dt: torch.tensor(list(a), dtype=dt).expand(rows).contiguous()  # noqa: E731
+    args = on(t, torch.float32), on(k, torch.int32), on(p, torch.float32), on(m, torch.float32)
+    ids, lps = pkg.sample_logits(logits, u.cuda(), *(a.cuda() for a in args))
+    host = logits.float().cpu().numpy()
+    for r in range(rows):
+        tr, kr, pr, mr = (a[r].item() for a in args)
+        keep, cum, lp = sample_reference(host[r], tr, kr, pr, mr)
+        most, _, _ = sample_reference(host[r], tr, kr, pr + 2.0 ** -21, mr)
+        i = ids[r].item()
+        assert i in most, (r, i, len(keep), len(most))
+        at = np.searchsorted(keep, i)
+        lo, hi = (cum[at - 1] if at else 0.0), cum[min(at, len(keep) - 1)]
+        assert lo - 2.0 ** -19 <= u[r].item() <= hi + 2.0 ** -19, (r, i, lo, hi, u[r].item())
+        assert abs(lps[r].item() - lp[i]) <= 2.0 ** -20 * (1 + abs(lp[i])), (r, lps[r].item(), lp[i])
+
+
+@pytest.mark.parametrize("vocab", [3000, 51866, 1 << 20])
+@pytest.mark.parametrize("depth", [15.0, 22.3, 26.0])
+def test_top_p_next_to_one_with_a_sure_token(pkg, vocab, depth):
+    # nearly all the weight on one token, a long tail far below it that top_p still cuts: the draws go to the tail's beginning, its cut
+    # and its end.  (2^20 tokens 26 nats below the sure one, each 2^-37 of it, hold 5e-6 of the weight.)
+    rows = 8
+    x = torch.full((rows, vocab), -depth)
+    x[:, 0] = 0.0
+    x[4:, 1::2] -= 0.5
+    tail = torch.exp(x[:, 1:].double()).sum(1)
+    for p in (0.9999, 0.99999, 0.999999, 1 - 2.0 ** -24):
+        for at in (0.0, 0.3, 0.9, 1.0):
+            u = ((1 + at * tail) / (1 + tail)).clamp_max(1 - 2.0 ** -53)
+            check_cut(pkg, x.cuda(), u, p=[p])
+        check_cut(pkg, x.cuda(), u, p=[p], t=[1.1], m=[1e-12])
+        check_cut(pkg, x.cuda(), u, p=[p], k=[vocab - 7])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_p_next_to_one(pkg, dtype):
+    g = torch.Generator().manual_seed(11)
+    x = 2 * torch.randn(12, 51866, generator=g)
+    x[::2, 77] = torch.tensor([25.0, 27.0, 29.0, 30.0, 31.0, 32.0])
+    x, u = x.to(dtype).cuda(), torch.rand(12, generator=g, dtype=torch.float64)
+    u[:6] = 1 - 2.0 ** -torch.arange(18, 42, 4, dtype=torch.float64)
+    for p in (0.9999, 0.999999, 1 - 2.0 ** -24):
+        check_cut(pkg, x, u, p=[p])
+        check_cut(pkg, x, u, p=[p], k=[20000])
+        check_cut(pkg, x, u, p=[p], k=[400], t=[0.7])
