@@ -53,8 +53,19 @@ struct Shared {
 struct Row {
     float max, c;  // c = log2(e) / temperature
     double c_d;
-    // -d = (x - max) log2(e) / temperature; -inf stays -inf.  Both roundings keep the order of the tokens.
-    __device__ __forceinline__ float power(float x) const { return (x - max) * c; }
+    float half, c2;  // -max / 2, 2 c
+    __device__ __forceinline__ void init(float max_, double temperature) {
+        max = max_;
+        // a temperature so small that its reciprocal overflows leaves the largest alone; an infinite one makes all tokens equal (in fp32
+        // to 10^-6 of a share, over the whole range of logits: -inf times 0 would be no number)
+        c_d = fmin(fmax(1.4426950408889634 / temperature, 0.0), 1e37);
+        c = fmaxf((float)c_d, 1.4e-45f);
+        half = -0.5f * max;
+        c2 = 2.0f * c;
+    }
+    // -d = (x - max) log2(e) / temperature; -inf stays -inf.  Both roundings keep the order of the tokens.  (By halves: the
+    // difference of two finite logits need not be finite.  The bits are the same where it is.)
+    __device__ __forceinline__ float power(float x) const { return fmaf(x, 0.5f, half) * c2; }
     __device__ __forceinline__ float share(float x) const { return __builtin_amdgcn_exp2f(power(x)); }  // of the likeliest token's probability
     // 2^43 of a share, to the nearest: 2^20 of them fit in 64 bits, and what 2^20 tokens of less than half a unit leave out is 2^-24 of the
     // likeliest one's (with 2^31 units top-p did not see tails that it has to cut)
@@ -493,10 +504,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs A) {
 #pragma unroll
     for (int w = 0; w < SW; ++w) mx = fmaxf(mx, S.wave_f[w]);
     Row R;
-    R.max = mx;
-    // an infinite temperature makes all tokens equal, one so small that its reciprocal overflows leaves the largest alone
-    R.c_d = fmin(fmax(1.4426950408889634 / (greedy ? 1.0 : (double)temp), 1e-30), 1e37);
-    R.c = (float)R.c_d;
+    R.init(mx, greedy ? 1.0 : (double)temp);
 
     // ---- 2: total weight; the likeliest tokens into a list, or a histogram ----
     const bool use_k = !greedy && k > 0 && k < A.n_vocab, use_p = !greedy && top_p < 1.0f, use_m = !greedy && min_p > 0.0f;

@@ -109,3 +109,17 @@ def test_top_p_next_to_one(pkg, dtype):
         check_cut(pkg, x, u, p=[p])
         check_cut(pkg, x, u, p=[p], k=[20000])
         check_cut(pkg, x, u, p=[p], k=[400], t=[0.7])
+
+
+@pytest.mark.parametrize("vocab", [300, 5000])
+def test_temperatures_for_logits_of_any_size(pkg, vocab):
+    # logits over the whole range of fp32 under temperatures of their size: their difference alone would leave the range
+    g = torch.Generator().manual_seed(vocab)
+    x = (torch.rand(8, vocab, generator=g) * 2 - 1) * 3e38
+    x[:, 3], x[:, 4], x[:, 5] = 3.4e38, -3.4e38, float("-inf")
+    u = torch.rand(8, generator=g, dtype=torch.float64)
+    t = [1e38, 3e38, 5e37, 1e31, float("inf"), 2e38, 1e36, 3.4e38]
+    check_sample(pkg, x.cuda(), u, t=t)
+    check_sample(pkg, x.cuda(), u, t=t, k=[20])
+    check_sample(pkg, x.cuda(), u, t=t, k=[vocab - 50], m=[1e-3])
+    check_sample(pkg, (x * 1e-7).cuda(), u, t=[a * 1e-7 for a in t])
