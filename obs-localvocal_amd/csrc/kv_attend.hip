@@ -597,7 +597,8 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             if (wave < 2) rs = sbase[pg * V.s_page + j * V.s_row];
         }
     };
-    // 8-bit rows: registers -> LDS, keys that no row sees as zeros; mark: the step, if some row may not see some key of it
+    // 8-bit rows: registers -> LDS, keys that no row sees as zeros; mark: the step, if some row may not see some key of it (the same
+    // steps here and at the end: what one leaves out the other adds)
     auto store = [&](int buf, int mark, unsigned long long gone) {
         bool bad = false;
 #pragma unroll
@@ -644,7 +645,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
         entry = entry_of(i0 + 1);
         if constexpr (!DIRECT) {
             __syncthreads();
-            store(0, all_see(key0) ? -1 : i0, dead);
+            store(0, dead == 0 && all_see(key0) ? -1 : i0, dead);
         }
     }
     arrived();
@@ -802,7 +803,7 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             if (!hide) products(cur, s);
         }
         if constexpr (!DIRECT) {
-            if (more) store(cur ^ 1, all_see(key1) ? -1 : i + 1, dead_n);
+            if (more) store(cur ^ 1, dead_n == 0 && all_see(key1) ? -1 : i + 1, dead_n);
         }
         dead = dead_n;
         cur ^= 1;

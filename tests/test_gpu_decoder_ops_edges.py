@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_decoder_ops import check_sample, sample_reference
+from test_gpu_decoder_ops import Case, check_attend, check_sample, sample_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,25 @@ def test_temperatures_for_logits_of_any_size(pkg, vocab):
     check_sample(pkg, x.cuda(), u, t=t, k=[20])
     check_sample(pkg, x.cuda(), u, t=t, k=[vocab - 50], m=[1e-3])
     check_sample(pkg, (x * 1e-7).cuda(), u, t=[a * 1e-7 for a in t])
+
+
+def poison(c, b, j, dim, value=float("nan")):
+    """A NaN code in one dim of the value at position j of sequence b (e4m3)."""
+    where = int(c.table[b, j // c.page]), slice(None), j % c.page, dim
+    c.codes[1][where] = value
+    c.cache.v.view(torch.uint8)[where] = 0x7f
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (400, 7)])
+def test_a_missing_page_and_a_nan_code_in_one_step(pkg, dim, window, sinks):
+    # a step of 64 keys that every row sees, with a page that is not there and a value that is no number in one dim, beside a step in which
+    # some rows do not see such a value: each key counts once, in the dims that are numbers
+    c = Case(pkg, "e4m3", dim, 2, 16, [160], [420], holes={(0, 5)})
+    poison(c, 0, 66, 9)    # keys 64 .. 127, of which page 5 (80 .. 95) is missing; all rows are behind them
+    poison(c, 0, 330, 20)  # the rows from position 330 on see it
+    q = torch.randn(160, 2, dim, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    out = c.cache.attend(q, c.batch, window=window, sinks=sinks)
+    check_attend(c, q, out, dim ** -0.5, window, sinks)
+    out = out.float().cpu()
+    assert torch.isnan(out[:, :, 9]).all() and torch.isnan(out[70:, :, 20]).all() and torch.isfinite(out[:70, :, 20]).all()
