@@ -771,6 +771,7 @@ def mx_layernorm(x, w, b, with_bf16=True, device=0):
 
 # ---- decoder operators on device memory (torch tensors; include/mi355_whisper.h says what they compute) ----
 # A call of a decode step is a few microseconds on the GPU, so the checks below are written to cost little on the way to it.
+# They serve inference: none has a gradient, and tensors that require one are refused while gradients are being recorded.
 
 _ELEM = {}  # torch dtype -> mw_elem
 _torch = None
@@ -816,6 +817,14 @@ def _rows(device, name, t, heads, head_dim, dtype=None):
 def _stream(device):
     """The current stream of a GPU (a hipStream_t)."""
     return _torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _no_gradient(what, *tensors):
+    """Refuses tensors whose gradient the caller expects: the operators have none, and a result without one would lose it in silence."""
+    if _torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient, and one of its tensors requires one: call it under torch.no_grad() or with detached tensors")
 
 
 def _call(what, rc):
@@ -880,6 +889,7 @@ class KvCache:
             raise ValueError("a bfloat16 cache has no scales")
         self.L, self.device, self.n_kv_heads, self.head_dim = lib(), d, k.shape[1], k.shape[3]
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._floats = (k, v) if e == ELEM_BF16 else (k_scale, v_scale)  # (codes cannot require a gradient)
         self.c = _KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
                           v_scale.data_ptr() if v_scale is not None else None, e, k.shape[0], k.shape[2], k.shape[1], k.shape[3],
                           k.stride(0), k.stride(1), k.stride(2), *s)
@@ -901,6 +911,7 @@ class KvCache:
         n = _rows(d, "k", k, self.n_kv_heads, self.head_dim)
         if _rows(d, "v", v, self.n_kv_heads, self.head_dim, k.dtype) != n:
             raise ValueError("k and v have to have one type, shape and layout")
+        _no_gradient("KvCache.write", k, v, *self._floats)
         _call("mw_kv_write_device", self.L.mw_kv_write_device(d.index, _stream(d), self._ref, C.byref(batch._for(d, n[0])), _elem(k), k.data_ptr(),
                                                               v.data_ptr(), n[1], n[2]))
 
@@ -915,6 +926,7 @@ class KvCache:
         n = _rows(d, "out[0]", k, self.n_kv_heads, self.head_dim, dtype)
         if _rows(d, "out[1]", v, self.n_kv_heads, self.head_dim, dtype) != n or n[0] != n_rows:
             raise ValueError("out has to be two tensors of n_rows rows in one type and layout")
+        _no_gradient("KvCache.read", k, v, *self._floats)
         _call("mw_kv_read_device", self.L.mw_kv_read_device(d.index, _stream(d), self._ref, C.byref(batch._for(d, n_rows)), _elem(k), k.data_ptr(),
                                                             v.data_ptr(), n[1], n[2]))
         return k, v
@@ -933,6 +945,7 @@ class KvCache:
             no, o_r, o_h = _rows(d, "out", out, heads, self.head_dim, bf16)
             if no != n:
                 raise ValueError("out has another number of rows than q")
+        _no_gradient("KvCache.attend", q, out, *self._floats)
         if window > 0x7fffffff or sinks > 0x7fffffff:  # (an int of C would take their low bits)
             raise ValueError(f"window {window} and sinks {sinks} have to be below 2^31")
         b = C.byref(batch._for(d, n))
@@ -967,5 +980,6 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
         if t.shape[0] != n or not t.is_contiguous():
             raise ValueError(f"{name} has to be contiguous with one entry per row")
         at.append(t.data_ptr())
+    _no_gradient("sample_logits", logits, temperature, top_p, min_p, u, out[1])
     _call("mw_sample_device", lib().mw_sample_device(d.index, _stream(d), logits.data_ptr(), _elem(logits), n, vocab, logits.stride(0), *at))
     return out

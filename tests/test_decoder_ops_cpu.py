@@ -108,3 +108,14 @@ def test_tensors_that_are_refused(pkg):
         pkg.KvBatch(i, i[:1], i[None])
     with pytest.raises(ValueError, match="one GPU"):
         pkg.sample_logits(torch.zeros(1, 8), torch.zeros(1, dtype=torch.float64))
+
+
+def test_gradients_are_refused_while_they_are_recorded(pkg):
+    pkg._load_torch()
+    t, p = torch.zeros(2), torch.zeros(2, requires_grad=True)
+    pkg._no_gradient("it", t, None)
+    with pytest.raises(RuntimeError, match="it has no gradient"):
+        pkg._no_gradient("it", t, None, p)
+    with torch.no_grad():
+        pkg._no_gradient("it", p)
+    pkg._no_gradient("it", p.detach())

@@ -145,3 +145,31 @@ def test_a_missing_page_and_a_nan_code_in_one_step(pkg, dim, window, sinks):
     check_attend(c, q, out, dim ** -0.5, window, sinks)
     out = out.float().cpu()
     assert torch.isnan(out[:, :, 9]).all() and torch.isnan(out[70:, :, 20]).all() and torch.isfinite(out[:70, :, 20]).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_tensors_that_require_gradients(pkg, kind):
+    # refused while gradients are recorded, taken under no_grad and when detached
+    c = Case(pkg, kind, 64, 2, 16, [3], [9])
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    x = torch.randn(3, 2, 64, device="cuda", requires_grad=True)
+    logits, u = torch.zeros(2, 40, device="cuda", requires_grad=True), torch.zeros(2, dtype=torch.float64, device="cuda")
+    before = c.cache.k.clone()
+    calls = [lambda g: c.cache.attend(g(q), c.batch), lambda g: c.cache.write(g(x), x.detach(), c.batch), lambda g: c.cache.write(x.detach(), g(x), c.batch),
+             lambda g: pkg.sample_logits(g(logits), u),
+             lambda g: pkg.sample_logits(logits.detach(), u, g(torch.ones(2, device="cuda", requires_grad=True)))]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(lambda t: t)
+    assert torch.equal(c.cache.k.view(torch.uint8), before.view(torch.uint8))
+    for t in c.cache._floats:
+        t.requires_grad_(True)
+        for call in (lambda: c.cache.attend(q.detach(), c.batch), lambda: c.cache.read(c.batch, 3, torch.float32),
+                     lambda: c.cache.write(x.detach(), x.detach(), c.batch)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        t.requires_grad_(False)
+    for call in calls:
+        call(lambda t: t.detach())
+        with torch.no_grad():
+            call(lambda t: t)
