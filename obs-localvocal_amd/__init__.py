@@ -848,6 +848,8 @@ class KvBatch:
             raise ValueError(f"cu_rows has {cu_rows.shape[0]} entries, kv_len {n}, block_table {tn} rows: n + 1, n and n are needed")
         if not (cu_rows.is_contiguous() and kv_len.is_contiguous()) or (cols > 1 and te != 1):
             raise ValueError("cu_rows, kv_len and the rows of block_table have to be contiguous")
+        if not (-0x80000000 <= max_rows <= 0x7fffffff and -0x80000000 <= max_kv <= 0x7fffffff):  # (as for attend's window)
+            raise ValueError(f"max_rows {max_rows} and max_kv {max_kv} have to be below 2^31")
         self.device, self.tensors = d, (cu_rows, kv_len, block_table)
         self.c = _KvBatch(n, 0, cu_rows.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), ts if ts > cols or n > 1 else cols, cols, max_rows, max_kv)
 
@@ -946,7 +948,7 @@ class KvCache:
             if no != n:
                 raise ValueError("out has another number of rows than q")
         _no_gradient("KvCache.attend", q, out, *self._floats)
-        if window > 0x7fffffff or sinks > 0x7fffffff:  # (an int of C would take their low bits)
+        if not (-0x80000000 <= window <= 0x7fffffff and -0x80000000 <= sinks <= 0x7fffffff):  # (an int of C would take their low bits)
             raise ValueError(f"window {window} and sinks {sinks} have to be below 2^31")
         b = C.byref(batch._for(d, n))
         need = self.L.mw_kv_attend_workspace(d.index, self._ref, b, heads, window, sinks)
@@ -965,6 +967,8 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     d = logits.device
     _on(d, "logits", logits, None, 2)
     n, vocab = logits.shape
+    if n > 0x7fffffff or vocab > 0x7fffffff:  # (as for attend's window)
+        raise ValueError(f"logits of {n} rows and {vocab} tokens: too many")
     if vocab > 1 and logits.stride(1) != 1:
         raise ValueError("the logits of a row have to be adjacent")
     if out is None:

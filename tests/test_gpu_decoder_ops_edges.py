@@ -173,3 +173,18 @@ def test_tensors_that_require_gradients(pkg, kind):
         call(lambda t: t.detach())
         with torch.no_grad():
             call(lambda t: t)
+
+
+def test_numbers_that_an_int_of_c_does_not_hold(pkg):
+    # their low bits would be legal numbers
+    c = Case(pkg, "bf16", 64, 2, 16, [3], [9])
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for window, sinks in ((5 - 2**32, 0), (5, 4 - 2**32), (2**32, 0), (2**31, 0)):
+        with pytest.raises(ValueError, match="below 2"):
+            c.cache.attend(q, c.batch, window=window, sinks=sinks)
+    for most in ((2**32 + 1, 9), (3, 2**32), (-2**32, 9)):
+        with pytest.raises(ValueError, match="below 2"):
+            pkg.KvBatch(*c.batch.tensors, *most)
+    wide = torch.zeros(8, device="cuda").expand(2**32 + 1, 8)
+    with pytest.raises(ValueError, match="too many"):
+        pkg.sample_logits(wide, torch.zeros(1, dtype=torch.float64, device="cuda"), out=(torch.zeros(1, dtype=torch.int32, device="cuda"),) * 2)
