@@ -113,7 +113,8 @@ int mw_process_logits(struct whisper_context *ctx, const struct whisper_full_par
 
    The cache.  Row `offset` of page `page` of head `h` is the head_dim consecutive elements at
    page * page_stride + h * head_stride + offset * row_stride of k and v, its scales the floats at the same place of
-   k_scale and v_scale with the scale strides.  Any order of pages, heads and rows is allowed.  head_dim is 64 or 128,
+   k_scale and v_scale with the scale strides.  Any order of pages, heads and rows is allowed; rows and scales that are written,
+   here and in the results below, may not overlap (strides smaller than a row are refused).  head_dim is 64 or 128,
    page_size a power of two up to 32768, strides multiples of 16 bytes and bases 16-byte aligned.  Element types:
      MW_ELEM_BF16  no scales
      MW_ELEM_E4M3  OCP e4m3 codes; scale = the smallest power of two >= 2^-126 with max|x| <= 448 scale

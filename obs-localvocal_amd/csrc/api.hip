@@ -866,7 +866,7 @@ int mw_kv_write_device(int device, void *stream, const struct mw_kv_cache *cache
                        const void *v, int64_t row_stride, int64_t head_stride) {
     if (!cache || !batch) return -1;
     return guarded("mw_kv_write_device", [&]() {
-        check_kv_rows(*cache, *batch, dtype, k, v, row_stride, head_stride);
+        check_kv_rows(*cache, *batch, dtype, k, v, row_stride, head_stride, true);
         OnDevice g(device);
         launch_kv_write(*cache, *batch, dtype, k, v, row_stride, head_stride, (hipStream_t)stream);
         return 0;
@@ -876,7 +876,7 @@ int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache,
                       int64_t row_stride, int64_t head_stride) {
     if (!cache || !batch) return -1;
     return guarded("mw_kv_read_device", [&]() {
-        check_kv_rows(*cache, *batch, dtype, k, v, row_stride, head_stride);
+        check_kv_rows(*cache, *batch, dtype, k, v, row_stride, head_stride, false);
         OnDevice g(device);
         launch_kv_read(*cache, *batch, dtype, k, v, row_stride, head_stride, (hipStream_t)stream);
         return 0;

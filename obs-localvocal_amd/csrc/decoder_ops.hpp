@@ -39,7 +39,8 @@ void launch_sample(const SampleArgs &a, hipStream_t st);
 
 // the checks of the arguments, on the host alone (throw with the reason)
 void check_kv(const mw_kv_cache &c, const mw_kv_batch &b);
-void check_kv_rows(const mw_kv_cache &c, const mw_kv_batch &b, int dtype, const void *k, const void *v, int64_t row_stride, int64_t head_stride);
+void check_kv_rows(const mw_kv_cache &c, const mw_kv_batch &b, int dtype, const void *k, const void *v, int64_t row_stride, int64_t head_stride,
+                   bool write);
 void check_kv_attend(const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendArgs &a);
 void check_sample(const SampleArgs &a);
 

@@ -999,6 +999,8 @@ void check_kv_attend(const mw_kv_cache &c, const mw_kv_batch &b, const KvAttendA
     MW_CHECK(a.q && a.out && ((uintptr_t)a.q | (uintptr_t)a.out) % 16 == 0 && a.q_row >= 0 && a.q_head >= 0 && a.o_row >= 0 && a.o_head >= 0 &&
                  a.q_row % 8 == 0 && a.q_head % 8 == 0 && a.o_row % 8 == 0 && a.o_head % 8 == 0,
              "kv attend: q and out pointers and strides are multiples of 16 bytes");
+    // (an expanded tensor has strides of 0: q may be one, out not)
+    MW_CHECK((b.n_rows == 1 || a.o_row >= c.head_dim) && (a.n_heads == 1 || a.o_head >= c.head_dim), "kv attend: the result's rows overlap");
     MW_CHECK((int64_t)b.n_rows * a.n_heads < (1LL << 26), "kv attend: too many rows");  // a grid holds 2^32 threads
 }
 

@@ -36,7 +36,8 @@ void check_kv(const mw_kv_cache &c, const mw_kv_batch &b) {
     MW_CHECK(b.max_rows >= 0 && b.max_kv >= 0, "kv batch: expected lengths");
 }
 
-void check_kv_rows(const mw_kv_cache &c, const mw_kv_batch &b, int dtype, const void *k, const void *v, int64_t row_stride, int64_t head_stride) {
+void check_kv_rows(const mw_kv_cache &c, const mw_kv_batch &b, int dtype, const void *k, const void *v, int64_t row_stride, int64_t head_stride,
+                   bool write) {
     check_kv(c, b);
     MW_CHECK(dtype == MW_ELEM_F32 || dtype == MW_ELEM_BF16, "kv rows: element type is f32 or bf16");
     if (b.n_rows == 0 || b.n_seqs == 0) return;
@@ -44,6 +45,17 @@ void check_kv_rows(const mw_kv_cache &c, const mw_kv_batch &b, int dtype, const 
     MW_CHECK(k && v && ((uintptr_t)k | (uintptr_t)v) % 16 == 0 && row_stride >= 0 && head_stride >= 0 && row_stride % al == 0 && head_stride % al == 0,
              "kv rows: pointers and strides are multiples of 16 bytes");
     MW_CHECK((int64_t)b.n_rows * c.n_kv_heads < (1LL << 28), "kv rows: too many rows");  // a grid holds 2^32 threads
+    // what is written must not share memory with itself (an expanded tensor has strides of 0); what is read may
+    auto apart = [](int64_t n, int64_t stride, int64_t least) { return n <= 1 || stride >= least; };
+    if (write) {
+        MW_CHECK(apart(c.n_pages, c.page_stride, c.head_dim) && apart(c.n_kv_heads, c.head_stride, c.head_dim) && apart(c.page_size, c.row_stride, c.head_dim),
+                 "kv rows: the cache's rows overlap");
+        MW_CHECK(c.dtype == MW_ELEM_BF16 || (apart(c.n_pages, c.scale_page_stride, 1) && apart(c.n_kv_heads, c.scale_head_stride, 1) &&
+                                             apart(c.page_size, c.scale_row_stride, 1)),
+                 "kv rows: the cache's scales overlap");
+    } else {
+        MW_CHECK(apart(b.n_rows, row_stride, c.head_dim) && apart(c.n_kv_heads, head_stride, c.head_dim), "kv rows: the result's rows overlap");
+    }
 }
 
 namespace {
@@ -240,7 +252,7 @@ __global__ __launch_bounds__(KT) void kv_rows_kernel(KvView V, const void *__res
 template <bool WRITE>
 void launch_rows(const mw_kv_cache &c, const mw_kv_batch &b, int dtype, const void *k, const void *v, void *kw, void *vw, int64_t row_stride,
                  int64_t head_stride, hipStream_t st) {
-    check_kv_rows(c, b, dtype, WRITE ? k : kw, WRITE ? v : vw, row_stride, head_stride);
+    check_kv_rows(c, b, dtype, WRITE ? k : kw, WRITE ? v : vw, row_stride, head_stride, WRITE);
     if (b.n_rows == 0 || b.n_seqs == 0) return;
     const KvView V = make_view(c, b);
     const int64_t items = (int64_t)b.n_rows * c.n_kv_heads;
