@@ -149,7 +149,8 @@ struct mw_kv_batch {
    and bases 16-byte aligned) -> the pages */
 int mw_kv_write_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int dtype,
                        const void *k, const void *v, int64_t row_stride, int64_t head_stride);
-/* the pages' contents at the batch's rows -> k, v (layout as above): code * scale, rounded once to dtype */
+/* the pages' contents at the batch's rows -> k, v (layout as above): the fp32 product code * scale, rounded to dtype (the bits of
+   tensor operations; of an int8 row in bf16 one element in 10^5 is a last place beside the exact product's rounding) */
 int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int dtype,
                       void *k, void *v, int64_t row_stride, int64_t head_stride);
 /* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the keys j of the row's sequence that its token sees: those at its
