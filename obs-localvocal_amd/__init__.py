@@ -819,12 +819,10 @@ def _stream(device):
     return _torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _no_gradient(what, *tensors):
-    """Refuses tensors whose gradient the caller expects: the operators have none, and a result without one would lose it in silence."""
+def _no_gradient(what):
+    """Refuses a call one of whose tensors requires a gradient: the operators have none, and a result without it would lose it in silence."""
     if _torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no gradient, and one of its tensors requires one: call it under torch.no_grad() or with detached tensors")
+        raise RuntimeError(f"{what} has no gradient, and one of its tensors requires one: call it under torch.no_grad() or with detached tensors")
 
 
 def _call(what, rc):
@@ -913,7 +911,9 @@ class KvCache:
         n = _rows(d, "k", k, self.n_kv_heads, self.head_dim)
         if _rows(d, "v", v, self.n_kv_heads, self.head_dim, k.dtype) != n:
             raise ValueError("k and v have to have one type, shape and layout")
-        _no_gradient("KvCache.write", k, v, *self._floats)
+        f, g = self._floats
+        if k.requires_grad or v.requires_grad or f.requires_grad or g.requires_grad:
+            _no_gradient("KvCache.write")
         _call("mw_kv_write_device", self.L.mw_kv_write_device(d.index, _stream(d), self._ref, C.byref(batch._for(d, n[0])), _elem(k), k.data_ptr(),
                                                               v.data_ptr(), n[1], n[2]))
 
@@ -928,7 +928,9 @@ class KvCache:
         n = _rows(d, "out[0]", k, self.n_kv_heads, self.head_dim, dtype)
         if _rows(d, "out[1]", v, self.n_kv_heads, self.head_dim, dtype) != n or n[0] != n_rows:
             raise ValueError("out has to be two tensors of n_rows rows in one type and layout")
-        _no_gradient("KvCache.read", k, v, *self._floats)
+        f, g = self._floats
+        if k.requires_grad or v.requires_grad or f.requires_grad or g.requires_grad:
+            _no_gradient("KvCache.read")
         _call("mw_kv_read_device", self.L.mw_kv_read_device(d.index, _stream(d), self._ref, C.byref(batch._for(d, n_rows)), _elem(k), k.data_ptr(),
                                                             v.data_ptr(), n[1], n[2]))
         return k, v
@@ -947,7 +949,9 @@ class KvCache:
             no, o_r, o_h = _rows(d, "out", out, heads, self.head_dim, bf16)
             if no != n:
                 raise ValueError("out has another number of rows than q")
-        _no_gradient("KvCache.attend", q, out, *self._floats)
+        f, g = self._floats
+        if q.requires_grad or out.requires_grad or f.requires_grad or g.requires_grad:
+            _no_gradient("KvCache.attend")
         if not (-0x80000000 <= window <= 0x7fffffff and -0x80000000 <= sinks <= 0x7fffffff):  # (an int of C would take their low bits)
             raise ValueError(f"window {window} and sinks {sinks} have to be below 2^31")
         b = C.byref(batch._for(d, n))
@@ -974,7 +978,7 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     if out is None:
         out = torch.empty(n, dtype=torch.int32, device=d), torch.empty(n, dtype=torch.float32, device=d)
     f32, i32 = torch.float32, torch.int32
-    at = []
+    at, grad = [], logits.requires_grad
     for name, t, kind in (("temperature", temperature, f32), ("top_k", top_k, i32), ("top_p", top_p, f32), ("min_p", min_p, f32), ("u", u, torch.float64),
                           ("out[0]", out[0], i32), ("out[1]", out[1], f32)):
         if t is None:
@@ -984,6 +988,8 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
         if t.shape[0] != n or not t.is_contiguous():
             raise ValueError(f"{name} has to be contiguous with one entry per row")
         at.append(t.data_ptr())
-    _no_gradient("sample_logits", logits, temperature, top_p, min_p, u, out[1])
+        grad |= t.requires_grad
+    if grad:
+        _no_gradient("sample_logits")
     _call("mw_sample_device", lib().mw_sample_device(d.index, _stream(d), logits.data_ptr(), _elem(logits), n, vocab, logits.stride(0), *at))
     return out
