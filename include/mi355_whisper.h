@@ -156,7 +156,8 @@ int mw_kv_read_device(int device, void *stream, const struct mw_kv_cache *cache,
 /* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the keys j of the row's sequence that its token sees: those at its
    position p and before it; with window > 0 only j > p - window and the first `sinks` positions.  Query head h reads key /
    value head h / (n_heads / n_kv_heads).  q and out: bf16, head h of row t at t * stride + h * head_stride, 16-byte aligned.
-   Scores, softmax and sums in fp32; the probabilities are rounded to bf16 for the product with v.  A row that sees nothing
+   Scores, softmax and sums in fp32; the probabilities are rounded to bf16 for the product with v, in calls of few rows a sequence
+   (single tokens, drafts) and over int8 caches with the rounding's residue.  A row that sees nothing, or only scores of -infinity,
    is zero.  Invisible keys and values are never used, whatever they hold.  scale > 0, finite.  workspace: at least
    mw_kv_attend_workspace bytes for the same device, cache, batch, n_heads, window and sinks (may be 0 bytes), 16-byte aligned. */
 size_t mw_kv_attend_workspace(int device, const struct mw_kv_cache *cache, const struct mw_kv_batch *batch, int n_heads, int window,
@@ -166,8 +167,9 @@ int mw_kv_attend_device(int device, void *stream, const struct mw_kv_cache *cach
                         int64_t out_head_stride, float scale, int window, int sinks, void *workspace, size_t workspace_bytes);
 /* One token per row of logits (MW_ELEM_F32 or MW_ELEM_BF16, [n_rows] rows row_stride elements apart).  x = logit / temperature[row];
    the tokens in the order (x falling, index rising); top_k keeps that many of them; top_p, of those, the fewest that hold
-   at least top_p of their probability (counted in 2^-43 of the likeliest token's); min_p, of those, the ones at least min_p times as likely as the likeliest; the token
-   is the first in the order of the index whose cumulated probability reaches u[row] (0 <= u < 1) of what is kept.
+   at least top_p of their probability (counted in 2^-43 of the likeliest token's); min_p, of those, the ones at least min_p times
+   as likely as the likeliest; the token is the first in the order of the index whose cumulated probability reaches u[row]
+   (0 <= u < 1) of what is kept.
    temperature <= 0: the first largest logit.  top_k <= 0, top_p >= 1 and min_p <= 0 keep all; the likeliest token is always
    kept.  The settings are device arrays [n_rows], each may be null (temperature 1, nothing dropped).  logprobs (may be null)
    gets log softmax(x) at the token over ALL tokens (as whisper_token_data.plog; temperature <= 0: x = logit).

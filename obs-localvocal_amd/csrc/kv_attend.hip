@@ -487,8 +487,9 @@ __global__ __launch_bounds__(64 * RW, DH == 64 ? 4 : 3) void attend_rows_kernel(
 //
 // Bound: the issue of the softmax's 5 operations a score beside the matrix products (which alone keep a wave busy for 40 % of a
 // step), so two or three workgroups a compute unit, one's softmax under another's products.  2048 tokens behind 14336, 32 heads on
-// 8 of 128, bf16: 555 us, 0.93 PFLOP/s (a plain product of 8192 cubed reaches 1.38); with rows through registers and pages looked
-// up beside their loads it was 640.  One half's exponents under the other's products took more registers than there are.  8 prompts
+// 8 of 128, bf16: 555 - 585 us from card to card, 0.9 PFLOP/s (a plain product of 8192 cubed reaches 1.38; calls back to back: traced
+// launches take 586 - 764); with rows through registers and pages looked up beside their loads it was 640 where it is 555 now.  8-bit
+// caches, whose codes each tile converts for itself: e4m3 688 us, int8 889 (a second product with the values) where bf16 takes 572.  One half's exponents under the other's products took more registers than there are.  8 prompts
 // of 17 - 448 tokens, 20 heads of 64: 32 us (64-row tiles), the longest tile's 23 steps.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int CR = 128, CK = 64;  // rows, keys per step
@@ -764,6 +765,10 @@ __global__ __launch_bounds__(256, DH == 64 && KIND == BF16 ? 3 : 2) void attend_
             if (c < 2 * NT - 1) fragments(c + 1, f[(c + 1) & 1]);
             const float *e = &s[c >> 1][8 * (c & 1)];
             const u32x4 pb = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
+            // A probability rounded to bf16 is off by at most 2^-8 of itself, as the result is when it is rounded: against the formula in 64
+            // bits the result is then off by 0.0020 - 0.0023 of its size, and by 0.0017 with the residue in a second product, which the
+            // 16-row kernel, waiting for memory, has for nothing.  Here it takes the chunk above from 555 to 745 us,
+            // the prompts from 30 to 33, chunks of 600 - 1777 rows under a window of 512 from 32 to 37.
             u32x4 pl = {0, 0, 0, 0};
             if constexpr (KIND == INT8) pl = low_part(e, pb);  // (a code's scale leaves the largest weight no power of two: its rounding would show)
 #pragma unroll

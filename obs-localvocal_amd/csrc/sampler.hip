@@ -2,7 +2,7 @@
 //
 // The order of the tokens of a row is never formed by sorting.  With x = logit / temperature and d = (max x - x) log2(e), a
 // token's weight is 2^-d.  Where weights are added in an order that may change (LDS atomics) they are whole numbers, so that
-// the sums are exact; the others are formed in one fixed order.  A token's place in the order is the 64-bit key
+// the sums are exact; the others are formed in one fixed order, in 64 bits beyond 16 bytes of a row (a tile of the draw: in fp32).  A token's place in the order is the 64-bit key
 // (falling logit, rising index), unique in the row.
 //   1. maximum of the row;
 //   2. total weight; when top-k or top-p cut, a histogram over d in 2048 bins (count and weight of each);
@@ -15,8 +15,9 @@
 // registers between the passes (56 a thread) the same code unrolled to 40 k instructions.
 // Bound: the latency of the passes one after the other, and in step 2 the histogram's LDS atomics (the same time with their branches
 // taken out).  f32, 51 866 tokens: one row with top-k 50, top-p and min-p 17 us (maximum 3, bound 1, total and list 5, two sorts and
-// the draw 3, launch); 64 rows of mixed settings 43 us, those with top-k 1000 and top-p the longest (histogram 10, a cut 9 each);
-// bf16, 128 000 tokens, 256 rows 75 us.  Loads of 64 bytes a thread at once changed none of them.
+// the draw 3, launch); 64 rows of mixed settings 46 us, those with top-k 1000 and top-p the longest (histogram 10, a cut 9 each);
+// bf16, 128 000 tokens, 256 rows 79 us, of which it reads 140 MB from memory: every row twice.  Loads of 64 bytes a thread at once
+// changed none of them.
 #include "decoder_ops.hpp"
 
 namespace mw {
